@@ -526,6 +526,144 @@ MQC_API int mqc_gate_residual_bwd(const void* z, int64_t z_row_stride, const voi
  * `out`: one device float, written only in a case that never occurs. */
 MQC_API int mqc_probe_fp32_fma(float* out, int64_t iters, int64_t* fmas_per_launch, void* stream);
 
+/* ---- gated linear recurrence (csrc/gated_scan.cu) -------------------------- */
+
+/* Over sequences [batch, seq_len, channels], s = sigmoid:
+ *   L[t] = sharpness softplus(lambda) s(r[t]),  a[t] = exp(-L[t]),
+ *   h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) s(i[t]) x[t],  y = h;
+ * where reset[t] != 0 the state is dropped: h[t] = s(i[t]) x[t].
+ * x, r, i: rows of `channels` contiguous elements at their own row strides
+ * (elements; row b * seq_len + t), dtype; y, dx, dr, di [batch, seq_len, channels]
+ * contiguous, dtype; lambda [channels], h0, hT, dhT, dh0 [batch, channels] fp32;
+ * reset [batch, seq_len] bytes or NULL. ckpt: states before every
+ * MQC_GATED_SCAN_TILE steps, [batch, ceil(seq_len / tile), channels] fp32: written
+ * by the forward pass when not NULL, read by the backward pass. h0, hT, dhT, dh0
+ * and dy may be NULL (zero, or not wanted). dlambda [channels] fp32.
+ * The reference has no real-valued recurrence. */
+#define MQC_GATED_SCAN_TILE 64
+typedef struct mqc_gated_scan_args {
+  int64_t batch, seq_len, channels;
+  int32_t dtype;
+  float sharpness;
+  const void *x, *r, *i;
+  int64_t x_row, r_row, i_row;
+  const void *lambda_, *h0, *reset;
+  void *y, *hT, *ckpt;
+  /* backward only */
+  const void *dy, *dhT;
+  int64_t dy_row;
+  void *dx, *dr, *di, *dlambda, *dh0;
+} mqc_gated_scan_args;
+MQC_API int mqc_gated_scan_fwd(const mqc_gated_scan_args* args, void* stream);
+
+/* Bytes of workspace mqc_gated_scan_bwd needs. */
+MQC_API size_t mqc_gated_scan_bwd_workspace_size(int64_t batch, int64_t seq_len,
+                                                 int64_t channels);
+/* Gradient of mqc_gated_scan_fwd; x, r, i, lambda, reset and ckpt as there.
+ * Fixed summation order. `workspace`: caller-owned, 4-byte aligned. */
+MQC_API int mqc_gated_scan_bwd(const mqc_gated_scan_args* args, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* One token of `batch` sequences: y[batch, channels] and h (fp32, in place). */
+MQC_API int mqc_gated_scan_step(const void* x, int64_t x_row, const void* r, int64_t r_row,
+                                const void* i, int64_t i_row, const void* lambda_, void* h,
+                                void* y, int64_t batch, int64_t channels, float sharpness,
+                                int dtype, void* stream);
+
+/* ---- norm + gate + residual (csrc/norm_gate.cu) ----------------------------- */
+
+/* Over rows of `width` columns, s = sigmoid:
+ *   out = x + scale * s(z) * P(y)      n = Q(out)
+ * P (weight, bias) and Q (next_weight, next_bias) are LayerNorm or RMSNorm over
+ * the row with the same eps. y NULL: no P, gate and residual, n = Q(x).
+ * next_weight NULL: no n. The biases may be NULL. x, out, dout, dx: x_dtype;
+ * y, z, n, dy, dz, dn: y_dtype (x fp32 with y bf16 is allowed, the reverse is
+ * not). All rows are contiguous, but z has a row stride of its own (elements).
+ * Parameters, their gradients and the per-row statistics are fp32; stats
+ * [rows, 4], 16-byte aligned, is written by the forward pass when not NULL and
+ * read by the backward pass. dout and dn may be NULL (zero); the column sums
+ * dweight .. dnext_bias may be NULL (not wanted). The forward pass is the
+ * reference's out_proj epilogue (models/quaternion_mamba2_block.py:154-164) with
+ * a norm on each side, which the reference does not have. */
+#define MQC_NORM_GATE_MAX_WIDTH 4096
+typedef enum mqc_norm { MQC_NORM_LAYER = 0, MQC_NORM_RMS = 1 } mqc_norm;
+typedef struct mqc_norm_gate_args {
+  int64_t rows, width, z_row;
+  int32_t x_dtype, y_dtype, norm;
+  float eps;
+  const void *x, *y, *z;
+  const float *weight, *bias, *scale, *next_weight, *next_bias;
+  void *out, *n, *stats;
+  /* backward only */
+  const void *dout, *dn;
+  void *dx, *dy, *dz;
+  float *dweight, *dscale, *dbias, *dnext_weight, *dnext_bias;
+} mqc_norm_gate_args;
+MQC_API int mqc_norm_gate_fwd(const mqc_norm_gate_args* args, void* stream);
+
+/* Bytes of workspace mqc_norm_gate_bwd needs. */
+MQC_API size_t mqc_norm_gate_bwd_workspace_size(int64_t rows, int64_t width);
+/* Gradient of mqc_norm_gate_fwd. Fixed summation order. `workspace`: caller-owned,
+ * 4-byte aligned. */
+MQC_API int mqc_norm_gate_bwd(const mqc_norm_gate_args* args, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* ---- optimizer: AdamW over a list of tensors (csrc/adamw.cu) --------------- */
+
+/* One AdamW step of `count` tensors:
+ *   m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2  (g times *clip),
+ *   p <- (1 - lr weight_decay) p - lr/(1 - beta1^step) m / (sqrt(v)/sqrt(1 - beta2^step) + eps).
+ * The lists are host arrays of `count` device pointers (contiguous tensors of
+ * numel[k] elements; a tensor of 0 elements is skipped and may be NULL).
+ * state_bits 32: exp_avg and exp_avg_sq are fp32. state_bits 8: exp_avg holds a
+ * byte an element (sign, 4 exponent and 3 fraction bits), exp_avg_sq a byte of
+ * sqrt(v) (4 exponent, 4 fraction bits), and the exponent lists one byte for each
+ * MQC_ADAMW_BLOCK elements (biased fp32 exponent of the block's largest value;
+ * 255 marks a block with a non-finite moment); all zero is a zero state. 8-bit
+ * moments and bf16 parameters are rounded up or down by a hash of seed, step,
+ * tensor and element. `clip`: device scalar (mqc_grad_norm's out + 1) or NULL.
+ * The reference trains with torch.optim.AdamW (train.py). */
+#define MQC_ADAMW_BLOCK 256
+/* 8-bit moments: a block whose largest value is above its power of two's last code
+ * takes the next power, instead of holding the value at that code. */
+#define MQC_ADAMW_CARRY 0x1
+typedef struct mqc_adamw_args {
+  int64_t count;
+  const int64_t* numel;
+  const int64_t* ordinal; /* hash ordinal of each tensor; NULL: its index */
+  void* const* param;
+  const void* const* grad;
+  void* const* exp_avg;
+  void* const* exp_avg_sq;
+  void* const* exp_avg_exponent;    /* 8 bits only */
+  void* const* exp_avg_sq_exponent; /* 8 bits only */
+  const float* clip;
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step; /* 1 for the first */
+  int32_t param_dtype, grad_dtype, state_bits, flags;
+  uint32_t seed, reserved0;
+} mqc_adamw_args;
+MQC_API int mqc_adamw_step(const mqc_adamw_args* args, void* stream);
+
+/* Values of 8-bit moments: out_avg[k] = m and out_root[k] = sqrt(v), bf16 (exact). */
+MQC_API int mqc_adamw_moments(int64_t count, const int64_t* numel, const void* const* exp_avg,
+                              const void* const* exp_avg_sq,
+                              const void* const* exp_avg_exponent,
+                              const void* const* exp_avg_sq_exponent, void* const* out_avg,
+                              void* const* out_root, void* stream);
+
+/* Bytes of workspace mqc_grad_norm needs for `count` tensors. */
+MQC_API size_t mqc_grad_norm_workspace_size(int64_t count);
+
+/* Euclidean norm of all gradients together: out[0] = norm (fp32),
+ * out[1] = min(1, max_norm / (norm + 1e-6)), 1 where max_norm < 0. dtype[k] is
+ * the mqc_dtype of grad[k]. Fixed summation order. `workspace`: caller-owned
+ * device memory, 8-byte aligned. Replaces clip_grad_norm_ (train.py:182-206)
+ * without its pass that scales the gradients. */
+MQC_API int mqc_grad_norm(int64_t count, const int64_t* numel, const void* const* grad,
+                          const int32_t* dtype, float max_norm, float* out, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

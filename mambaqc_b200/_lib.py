@@ -84,6 +84,68 @@ class BcProjScanArgs(ctypes.Structure):
     ]
 
 
+MQC_GATED_SCAN_TILE = 64
+
+
+class GatedScanArgs(ctypes.Structure):
+    """Mirror of ``mqc_gated_scan_args``."""
+
+    _fields_ = [
+        ("batch", _i64), ("seq_len", _i64), ("channels", _i64),
+        ("dtype", ctypes.c_int32), ("sharpness", _f32),
+        ("x", _c_void_p), ("r", _c_void_p), ("i", _c_void_p),
+        ("x_row", _i64), ("r_row", _i64), ("i_row", _i64),
+        ("lambda_", _c_void_p), ("h0", _c_void_p), ("reset", _c_void_p),
+        ("y", _c_void_p), ("hT", _c_void_p), ("ckpt", _c_void_p),
+        ("dy", _c_void_p), ("dhT", _c_void_p), ("dy_row", _i64),
+        ("dx", _c_void_p), ("dr", _c_void_p), ("di", _c_void_p), ("dlambda", _c_void_p),
+        ("dh0", _c_void_p),
+    ]
+
+
+MQC_NORM_GATE_MAX_WIDTH = 4096
+MQC_NORM_LAYER = 0
+MQC_NORM_RMS = 1
+
+
+class NormGateArgs(ctypes.Structure):
+    """Mirror of ``mqc_norm_gate_args``."""
+
+    _fields_ = [
+        ("rows", _i64), ("width", _i64), ("z_row", _i64),
+        ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("norm", ctypes.c_int32),
+        ("eps", _f32),
+        ("x", _c_void_p), ("y", _c_void_p), ("z", _c_void_p),
+        ("weight", _c_void_p), ("bias", _c_void_p), ("scale", _c_void_p),
+        ("next_weight", _c_void_p), ("next_bias", _c_void_p),
+        ("out", _c_void_p), ("n", _c_void_p), ("stats", _c_void_p),
+        ("dout", _c_void_p), ("dn", _c_void_p),
+        ("dx", _c_void_p), ("dy", _c_void_p), ("dz", _c_void_p),
+        ("dweight", _c_void_p), ("dscale", _c_void_p), ("dbias", _c_void_p),
+        ("dnext_weight", _c_void_p), ("dnext_bias", _c_void_p),
+    ]
+
+
+MQC_ADAMW_BLOCK = 256
+MQC_ADAMW_CARRY = 0x1
+
+
+class AdamwArgs(ctypes.Structure):
+    """Mirror of ``mqc_adamw_args`` (the lists are ctypes arrays of pointers)."""
+
+    _fields_ = [
+        ("count", _i64), ("numel", _c_void_p), ("ordinal", _c_void_p),
+        ("param", _c_void_p), ("grad", _c_void_p), ("exp_avg", _c_void_p),
+        ("exp_avg_sq", _c_void_p), ("exp_avg_exponent", _c_void_p),
+        ("exp_avg_sq_exponent", _c_void_p), ("clip", _c_void_p),
+        ("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double),
+        ("step", _i64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32), ("flags", ctypes.c_int32), ("seed", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
 # name -> (argtypes); every function returns int status unless listed in _STR_FUNCS
 _SIGNATURES = {
     "mqc_qmul": [_c_void_p, _c_void_p, _c_void_p, _i64, _i32, _c_void_p],
@@ -145,11 +207,26 @@ _SIGNATURES.update({
     "mqc_channel_push": [_c_void_p, ctypes.POINTER(_c_void_p), _i32, _i64, _i64, _i64, _i64,
                          _i64, _i64, _i64, _i32, _c_void_p],
 })
+_SIGNATURES.update({
+    "mqc_gated_scan_fwd": [ctypes.POINTER(GatedScanArgs), _c_void_p],
+    "mqc_gated_scan_bwd": [ctypes.POINTER(GatedScanArgs), _c_void_p, ctypes.c_size_t, _c_void_p],
+    "mqc_gated_scan_step": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                            _c_void_p, _c_void_p, _i64, _i64, _f32, _i32, _c_void_p],
+    "mqc_norm_gate_fwd": [ctypes.POINTER(NormGateArgs), _c_void_p],
+    "mqc_norm_gate_bwd": [ctypes.POINTER(NormGateArgs), _c_void_p, ctypes.c_size_t, _c_void_p],
+    "mqc_adamw_step": [ctypes.POINTER(AdamwArgs), _c_void_p],
+    "mqc_adamw_moments": [_i64] + [_c_void_p] * 8,
+    "mqc_grad_norm": [_i64, _c_void_p, _c_void_p, _c_void_p, _f32, _c_void_p, _c_void_p,
+                      ctypes.c_size_t, _c_void_p],
+})
 MQC_PEER_HANDLE_BYTES = 64
 _SIZE_FUNCS = {"mqc_qln_bwd_workspace_size": [_i64, _i64],
                "mqc_ssm_scan_fwd_chunked_workspace_size": [_i64, _i64, _i64, _i64],
                "mqc_conv_silu_bwd_workspace_size": [_i64, _i64, _i64, _i64],
-               "mqc_ssm_scan_fwd_summary_workspace_size": [_i64, _i64, _i64, _i64]}
+               "mqc_ssm_scan_fwd_summary_workspace_size": [_i64, _i64, _i64, _i64],
+               "mqc_gated_scan_bwd_workspace_size": [_i64, _i64, _i64],
+               "mqc_norm_gate_bwd_workspace_size": [_i64, _i64],
+               "mqc_grad_norm_workspace_size": [_i64]}
 _STR_FUNCS = {"mqc_version": [], "mqc_status_string": [_i32], "mqc_last_error": []}
 
 _lock = threading.Lock()
@@ -199,6 +276,16 @@ def check(rc: int, what: str) -> None:
 def call(name: str, *args) -> None:
     lib = load()
     check(getattr(lib, name)(*args), name)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device`` current and its current stream as the last argument."""
+    idx = device.index
+    if idx is None or idx == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -10,6 +10,9 @@ reference trainer without gradient accumulation:
 - forward with labels under bf16 autocast, then backward (train.py:154-180);
 - clipping at ``grad_clip``, the optimizer step and zeroing the gradients
   (train.py:182-206).
+
+Any ``torch.optim`` optimizer serves; with ``mambaqc_b200.optim.AdamW`` clipping and
+update run in a few launches over all tensors, and its moments can be held in 8 bits.
 """
 
 from __future__ import annotations
@@ -17,6 +20,8 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel
+
+from mambaqc_b200.optim import AdamW
 
 __all__ = ["data_parallel", "train_step"]
 
@@ -47,6 +52,10 @@ def train_step(model: torch.nn.Module, optimizer: torch.optim.Optimizer,
     else:
         loss = model(input_ids, labels=labels)["loss"]
     loss.backward()
+    if isinstance(optimizer, AdamW):
+        # clipping is part of its step: no pass that rewrites the gradients
+        optimizer.step(max_grad_norm=grad_clip if grad_clip and grad_clip > 0 else None)
+        return loss.detach()
     if grad_clip is not None and grad_clip > 0:
         torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)
     optimizer.step()
