@@ -1,4 +1,5 @@
-"""Models: drop-ins for the block and the LM wrapper of ``mambaqc.models``."""
+"""Models: drop-ins for the block and the LM wrapper of ``mambaqc.models``, and a normed
+stack of gated recurrent and quaternion blocks."""
 
 from .quaternion_mamba2_block import QuaternionMamba2Block
 from .quaternion_mamba2 import (
@@ -7,6 +8,7 @@ from .quaternion_mamba2 import (
     quaternion_mamba2_large,
     quaternion_mamba2_small,
 )
+from .gated_recurrent import GatedRecurrentBlock, HybridMamba2
 
 __all__ = [
     "QuaternionMamba2Block",
@@ -14,4 +16,6 @@ __all__ = [
     "quaternion_mamba2_small",
     "quaternion_mamba2_base",
     "quaternion_mamba2_large",
+    "GatedRecurrentBlock",
+    "HybridMamba2",
 ]

@@ -66,17 +66,21 @@ class QuaternionMamba2(nn.Module):
             nn.init.ones_(module.weight)
             nn.init.zeros_(module.bias)
 
-    def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None):
-        assert input_ids.min() >= 0, f"Negative token index: {input_ids.min().item()}"
-        assert input_ids.max() < self.vocab_size, \
-            f"Token index {input_ids.max().item()} >= vocab_size {self.vocab_size}"
+    def _features(self, input_ids: torch.Tensor) -> torch.Tensor:
+        """What the head reads: the normed output of the last layer."""
         x = self.dropout(self.embedding(input_ids))
         for layer in self.layers:
             if self.gradient_checkpointing and self.training and torch.is_grad_enabled():
                 x = ckpt.checkpoint(layer, x, use_reentrant=False)
             else:
                 x = layer(x)
-        logits = self.lm_head(self.norm_f(x))[..., : self.vocab_size]
+        return self.norm_f(x)
+
+    def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None):
+        assert input_ids.min() >= 0, f"Negative token index: {input_ids.min().item()}"
+        assert input_ids.max() < self.vocab_size, \
+            f"Token index {input_ids.max().item()} >= vocab_size {self.vocab_size}"
+        logits = self.lm_head(self._features(input_ids))[..., : self.vocab_size]
         loss = None
         if labels is not None:
             valid = labels[labels != -100]

@@ -93,14 +93,20 @@ class QuaternionMamba2Block(nn.Module):
 
     def forward(self, x: torch.Tensor, return_ssm_state: bool = False,
                 fused_bc_proj: bool | None = None):
+        y_real, z, h_T = self.mix(x, fused_bc_proj=fused_bc_proj)
+        out = gate_residual(x, z, y_real)
+        return (out, h_T) if return_ssm_state else out
+
+    def mix(self, x: torch.Tensor, fused_bc_proj: bool | None = None):
+        """The block without its output gate and residual: (y_real, z, h_T), with
+        ``forward(x) = gate_residual(x, z, y_real)``. For stacks that put their own
+        norms around a block (``norm_gate_residual``)."""
         xz = self.in_proj(x)
         x_inner, z = xz.chunk(2, dim=-1)
         conv = self.conv1d.conv
         x_act = causal_conv1d_silu(x_inner, conv.weight, conv.bias)
         y_quat, h_T = self._ssm_forward(x_act, return_state=True, fused_bc_proj=fused_bc_proj)
-        y_real = self._norm_out_proj(y_quat)
-        out = gate_residual(x, z[..., : self.d_model], y_real)
-        return (out, h_T) if return_ssm_state else out
+        return self._norm_out_proj(y_quat), z[..., : self.d_model], h_T
 
     def _norm_out_proj(self, y_quat: torch.Tensor) -> torch.Tensor:
         """``out_proj(norm(y_quat))`` (block lines 154-157). With
@@ -162,13 +168,22 @@ class QuaternionMamba2Block(nn.Module):
         [B, d_conv-1, d_inner] (zeros before the start), "h": the SSM state
         [B, d_inner, d_state, 4] fp32}."""
         out, h_T = self.forward(x, return_ssm_state=True)
+        return out, self._cache(x, h_T)
+
+    def _cache(self, x: torch.Tensor, h_T: torch.Tensor) -> dict:
         k1 = self.d_conv - 1
         x_inner = self.in_proj(x)[..., : self.d_inner]
         hist = x_inner.new_zeros(x.shape[0], k1, self.d_inner)
         take = min(k1, x.shape[1])
         if take > 0:
             hist[:, k1 - take:] = x_inner[:, -take:]
-        return out, {"conv": hist, "h": h_T.contiguous()}
+        return {"conv": hist, "h": h_T.contiguous()}
+
+    @torch.no_grad()
+    def mix_prefill(self, x: torch.Tensor):
+        """``mix`` over a prompt with the cache of ``prefill``: (y_real, z, cache)."""
+        y_real, z, h_T = self.mix(x)
+        return y_real, z, self._cache(x, h_T)
 
     @torch.no_grad()
     def step(self, x_t: torch.Tensor, cache: dict) -> torch.Tensor:
@@ -177,6 +192,12 @@ class QuaternionMamba2Block(nn.Module):
         inputs plus this one, and the SSM advances its state in place
         (``ssm_step_cayley``). Same result as running the whole sequence
         through ``forward`` and taking the last position."""
+        y_real, z = self.mix_step(x_t, cache)
+        return gate_residual(x_t, z, y_real)
+
+    @torch.no_grad()
+    def mix_step(self, x_t: torch.Tensor, cache: dict):
+        """``step`` without the output gate and residual: (y_real, z) of one token."""
         bsz = x_t.shape[0]
         xz = self.in_proj(x_t)
         x_in, z = xz.chunk(2, dim=-1)
@@ -191,8 +212,7 @@ class QuaternionMamba2Block(nn.Module):
         y = ssm_step_cayley(delta.to(dt).contiguous(), self.ssm_lambda(), Bq.contiguous(),
                             Cq.to(dt).contiguous(), s_real.to(dt).contiguous(), self.D,
                             cache["h"])
-        y_real = self.out_proj(self.norm(y[:, None]))[:, 0]
-        return gate_residual(x_t, z[..., : self.d_model], y_real)
+        return self.out_proj(self.norm(y[:, None]))[:, 0], z[..., : self.d_model]
 
     def extra_repr(self) -> str:
         return (f"d_model={self.d_model}, d_state={self.d_state}, d_inner={self.d_inner}, "
