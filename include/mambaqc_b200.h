@@ -553,6 +553,7 @@ typedef struct mqc_gated_scan_args {
   const void *dy, *dhT;
   int64_t dy_row;
   void *dx, *dr, *di, *dlambda, *dh0;
+  void* status; /* device int32 or NULL: a bounded wait that gave up */
 } mqc_gated_scan_args;
 MQC_API int mqc_gated_scan_fwd(const mqc_gated_scan_args* args, void* stream);
 

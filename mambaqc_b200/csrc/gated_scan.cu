@@ -43,7 +43,10 @@ using pk::neg2;
 
 constexpr int kChan = 64;  // channels of a CTA
 constexpr int kTile = MQC_GATED_SCAN_TILE;  // time steps of a tile
-constexpr int kMaxCluster = 16;
+// CTAs of a cluster: as many as the exchange's shared memory leaves room for two CTAs
+// an SM beside (16 is the device's limit, above the portable 8)
+template <typename T>
+constexpr int kMaxCluster = sizeof(T) == 2 ? 16 : 8;
 
 // ---------------------------------------------------------------- arithmetic
 
@@ -126,16 +129,14 @@ __device__ __forceinline__ float2 join_decay(float2 M, float2 m) {
   return add2(M, fma2(M, m, m));
 }
 
+__device__ __forceinline__ float join_decay(float M, float m) { return M + fmaf(M, m, m); }
+
 // A s + E with A = 1 + M. kDrop: where M is -1 (a reset) s is dropped, also if it is
 // infinite or NaN.
 template <bool kDrop>
-__device__ __forceinline__ float2 apply(float2 M, float2 E, float2 s) {
-  float2 r = add2(s, fma2(M, s, E));
-  if (kDrop) {
-    if (M.x == -1.f) r.x = E.x;
-    if (M.y == -1.f) r.y = E.y;
-  }
-  return r;
+__device__ __forceinline__ float apply(float M, float E, float s) {
+  const float r = s + fmaf(M, s, E);
+  return kDrop && M == -1.f ? E : r;
 }
 
 // 1 / sqrt(q); 0 where q is 0 or subnormal (no decay to speak of: neither the
@@ -147,74 +148,68 @@ __device__ __forceinline__ float2 inv_sqrt2(float2 q) {
 
 // ------------------------------------------------------------------- memory
 
-// Two channels of one row as they are stored: one word of adjacent channels (kVec)
-// or two elements 32 channels apart (any width and alignment).
-template <typename T, bool kVec>
-struct Pair;
-
-template <>
-struct Pair<float, true> {
-  float2 v;
-  __device__ __forceinline__ void load(const float* p, int, bool, bool) {
-    v = __ldg(reinterpret_cast<const float2*>(p));
-  }
-  __device__ __forceinline__ float2 get() const { return v; }
-  static __device__ __forceinline__ void store(float* p, float2 o, int, bool, bool) {
-    *reinterpret_cast<float2*>(p) = o;
-  }
-};
-template <>
-struct Pair<__nv_bfloat16, true> {
-  uint32_t v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, int, bool, bool) {
-    v = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
-  __device__ __forceinline__ float2 get() const {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, float2 o, int, bool, bool) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(o.x, o.y);
-    *reinterpret_cast<__nv_bfloat162*>(p) = h;
-  }
-};
-template <typename T>
-struct Pair<T, false> {
-  T a, b;
-  __device__ __forceinline__ void load(const T* p, int step, bool ok0, bool ok1) {
-    a = ok0 ? __ldg(p) : T(0.f);
-    b = ok1 ? __ldg(p + step) : T(0.f);
-  }
-  __device__ __forceinline__ float2 get() const { return make_float2(to_f(a), to_f(b)); }
-  static __device__ __forceinline__ void store(T* p, float2 o, int step, bool ok0, bool ok1) {
-    if (ok0) QIO<T>::st1(p, o.x);
-    if (ok1) QIO<T>::st1(p + step, o.y);
-  }
-};
-
-// The two channels of a lane: columns c and c + step of the tensors.
-struct Lane {
-  int c, step;
-  bool ok0, ok1;
-};
-
+// Two adjacent channels. kVec: the pair is one aligned word of the tensor.
+__device__ __forceinline__ float2 unpack2(const float* p) {
+  return *reinterpret_cast<const float2*>(p);
+}
+__device__ __forceinline__ float2 unpack2(const __nv_bfloat16* p) {
+  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 template <bool kVec>
-__device__ __forceinline__ Lane lane_of(int tile, int channels) {
-  const int l = threadIdx.x & 31;
-  Lane r;
-  r.step = kVec ? 1 : 32;
-  r.c = tile * kChan + (kVec ? 2 * l : l);
-  r.ok0 = r.c < channels;
-  r.ok1 = r.c + r.step < channels;
-  return r;
+__device__ __forceinline__ void store2(float* p, float2 o, bool ok0, bool ok1) {
+  if (kVec) {
+    if (ok0) *reinterpret_cast<float2*>(p) = o;
+  } else {
+    if (ok0) p[0] = o.x;
+    if (ok1) p[1] = o.y;
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float2 o, bool ok0, bool ok1) {
+  if (kVec) {
+    if (ok0) *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(o.x, o.y);
+  } else {
+    if (ok0) p[0] = __float2bfloat16_rn(o.x);
+    if (ok1) p[1] = __float2bfloat16_rn(o.y);
+  }
 }
 
-__device__ __forceinline__ float2 load_f2(const float* p, const Lane& l) {
-  if (p == nullptr) return bc2(0.f);
-  return make_float2(l.ok0 ? p[l.c] : 0.f, l.ok1 ? p[l.c + l.step] : 0.f);
+// One tile (kTile rows of kChan channels) of a tensor into shared memory. kBytes: what
+// one copy moves (16 or 4: cp.async; else single elements through registers). Rows
+// from `rows` on and channels from `cols` on become zero and are not read. `src`: the
+// tile's first element, or NULL for zeros.
+template <typename T, int kBytes, int kThreads>
+__device__ __forceinline__ void copy_tile(T* dst, const T* src, int64_t stride, int rows, int cols) {
+  constexpr int kPer = kBytes / int(sizeof(T));  // elements a copy
+  constexpr int kUnits = kChan / kPer;           // copies a row
+  constexpr int kEach = kTile * kUnits / kThreads;
+  static_assert(kTile * kUnits % kThreads == 0 && kThreads % kUnits == 0, "whole rounds");
+  const int unit = int(threadIdx.x) % kUnits, row0 = int(threadIdx.x) / kUnits;
+  const int c = unit * kPer;
+  const int have = min(max(cols - c, 0), kPer) * int(sizeof(T));
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int row = row0 + k * (kThreads / kUnits);
+    const int bytes = row < rows && src != nullptr ? have : 0;
+    T* d = dst + row * kChan + c;
+    if constexpr (kBytes == 16) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(d)),
+                   "l"(bytes ? src + row * stride + c : src), "r"(bytes)
+                   : "memory");
+    } else if constexpr (kBytes == 4) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(d)),
+                   "l"(bytes ? src + row * stride + c : src), "r"(bytes)
+                   : "memory");
+    } else {
+      *d = bytes ? __ldg(src + row * stride + c) : T(0.f);
+    }
+  }
 }
-__device__ __forceinline__ void store_f2(float* p, float2 v, const Lane& l) {
-  if (l.ok0) p[l.c] = v.x;
-  if (l.ok1) p[l.c + l.step] = v.y;
+
+__device__ __forceinline__ float2 load_f2(const float* p, int c, bool ok0, bool ok1) {
+  if (p == nullptr) return bc2(0.f);
+  return make_float2(ok0 ? p[c] : 0.f, ok1 ? p[c + 1] : 0.f);
 }
 
 struct FwdArgs {
@@ -226,6 +221,7 @@ struct FwdArgs {
   void* y;
   float* hT;
   float* ckpt;  // [batch][tiles][channels]: state before each tile, or NULL
+  int* status;
   int batch, seq, channels, chan_tiles;
   float sharpness;
 };
@@ -240,306 +236,402 @@ struct BwdArgs {
   void *dx, *dr, *di;
   float* dh0;
   float* part;  // [batch][channels] x cluster rank: sums of dL s(r)
+  int* status;
   int batch, seq, channels, chan_tiles;
   float sharpness;
 };
+
+// --------------------------------------------------- exchange between the CTAs
+
+// What one thread a channel of each CTA tells all CTAs of its cluster in a round: the
+// pair (M, E) of its tile, written into their shared memory with the bytes counted on
+// an mbarrier there, so a round needs no barrier of the cluster and no fence that
+// waits for the global stores in flight. Two buffers in turn: a CTA writes round k + 2
+// only after it has every message of round k + 1, which their senders sent after
+// they had read round k.
+template <int kRanks>
+struct Exchange {
+  float2 sum[2][kRanks][kChan];
+  uint64_t bar[2];
+};
+constexpr int kPollLimit = 1 << 22;  // then the wait is given up and reported
+
+template <int kRanks>
+__device__ __forceinline__ void exchange_init(Exchange<kRanks>* x) {
+  if (threadIdx.x == 0) {
+    mbar_init(&x->bar[0], 1);
+    mbar_init(&x->bar[1], 1);
+    fence_mbar_init();
+  }
+}
+
+__device__ __forceinline__ uint32_t remote_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+// Sends this channel's pair and waits for those of all ranks; false: given up.
+template <int kRanks>
+__device__ __forceinline__ bool exchange(Exchange<kRanks>* x, int buf, uint32_t parity, int rank, int csize,
+                                         int ch, float m, float e, int* status) {
+  if (ch == 0) mbar_arrive_expect_tx(&x->bar[buf], uint32_t(csize * kChan * sizeof(float2)));
+  const uint32_t at = smem_addr(&x->sum[buf][rank][ch]), bar = smem_addr(&x->bar[buf]);
+  for (int to = 0; to < csize; ++to)
+    asm volatile(
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::
+            "r"(remote_addr(at, to)),
+        "f"(m), "f"(e), "r"(remote_addr(bar, to))
+        : "memory");
+  for (int k = 0; k < kPollLimit; ++k) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  report_status(status, MQC_DEVICE_STATUS_TIMEOUT);
+  return false;
+}
 
 // ------------------------------------------------------------------- forward
 
 constexpr int kFwdWarps = 8;
 
-template <typename T, bool kVec, bool kReset>
-__global__ void __launch_bounds__(kFwdWarps * 32)
+template <typename T>
+struct FwdSmem {
+  T raw[2][3][kTile][kChan];          // x, r, i of this tile and the next
+  float2 run[kFwdWarps][kChan];       // (M, E) of each warp's run
+  float start[kFwdWarps][kChan];      // state before each run
+  Exchange<kMaxCluster<T>> ex;
+};
+
+// One tile: (A) each warp reduces its run to (M, E); (B) one thread a channel joins
+// the runs, exchanges the tile's pair with the cluster and hands each run its start;
+// (C) each warp runs its steps again from there and stores y. The next tile's copies
+// are in flight meanwhile.
+template <typename T, int kBytes, bool kVec, bool kReset>
+__global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     gated_scan_fwd_kernel(const FwdArgs p) {
-  constexpr int W = kFwdWarps, S = kTile / W;
-  // (A0, A1, E0, E1) of each warp's run and of each CTA's tile, double-buffered
-  __shared__ float4 seg[2][W][32];
-  __shared__ float4 sum[2][kMaxCluster][32];
+  constexpr int W = kFwdWarps, S = kTile / W, kThreads = W * 32;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  FwdSmem<T>& sm = *reinterpret_cast<FwdSmem<T>*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int unit = int(blockIdx.x) / csize;
   const int b = unit / p.chan_tiles;
-  const Lane ln = lane_of<kVec>(unit - b * p.chan_tiles, p.channels);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = (unit - b * p.chan_tiles) * kChan;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int c = c0 + 2 * lane;
+  const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
   const int tiles = (p.seq + kTile - 1) / kTile;
   const int64_t row0 = int64_t(b) * p.seq;
-  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + ln.c;
-  const T* r = static_cast<const T*>(p.r) + row0 * p.rs + ln.c;
-  const T* iv = static_cast<const T*>(p.i) + row0 * p.is + ln.c;
-  T* y = static_cast<T*>(p.y) + row0 * p.channels + ln.c;
+  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + c0;
+  const T* r = static_cast<const T*>(p.r) + row0 * p.rs + c0;
+  const T* iv = static_cast<const T*>(p.i) + row0 * p.is + c0;
+  T* y = static_cast<T*>(p.y) + row0 * p.channels + c;
   const uint8_t* rst = kReset ? p.reset + row0 : nullptr;
-  const float2 lam = load_f2(p.lambda, ln);
+  const float2 lam = load_f2(p.lambda, c, ok0, ok1);
   const float2 rate = make_float2(p.sharpness * softplus_acc(lam.x), p.sharpness * softplus_acc(lam.y));
-  float2 carry = load_f2(p.h0 ? p.h0 + int64_t(b) * p.channels : nullptr, ln);
+  // the joining threads' channel and its state, passed from round to round
+  const int jc = c0 + tid;
+  const bool jok = tid < kChan && jc < p.channels;
+  float carry = jok && p.h0 ? p.h0[int64_t(b) * p.channels + jc] : 0.f;
 
-  Pair<T, kVec> xr[S], rr[S], ir[S];
-  bool rs[S];
-  auto load = [&](int tile) {
-    const int t0 = tile * kTile + warp * S;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int t = t0 + s;
-      const bool in = t < p.seq;
-      if (kReset) rs[s] = in && rst[t] != 0;
-      if (in && ln.ok0) {
-        xr[s].load(x + t * p.xs, ln.step, ln.ok0, ln.ok1);
-        rr[s].load(r + t * p.rs, ln.step, ln.ok0, ln.ok1);
-        ir[s].load(iv + t * p.is, ln.step, ln.ok0, ln.ok1);
-      } else {
-        xr[s] = rr[s] = ir[s] = Pair<T, kVec>{};
-      }
-    }
+  auto load = [&](int tile, int st) {
+    const int64_t t0 = int64_t(tile) * kTile;
+    const int rows = p.seq - int(t0), cols = p.channels - c0;
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][0][0][0], x + t0 * p.xs, p.xs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][1][0][0], r + t0 * p.rs, p.rs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][2][0][0], iv + t0 * p.is, p.is, rows, cols);
   };
 
-  load(rank);
-  if (csize > 1) cluster.sync();  // every CTA has begun before its shared memory is written
-  int buf = 0;
-  for (int first = 0; first < tiles; first += csize, buf ^= 1) {
-    const int tile = first + rank;
+  if (csize > 1) exchange_init(&sm.ex);
+  if (rank < tiles) load(rank, 0);
+  cp_async_commit();
+  if (csize > 1) cluster.sync();  // every CTA's mbarriers are ready before they are written
+  bool alive = true;
+  int round = 0;
+  for (int first = 0; first < tiles; first += csize, ++round) {
+    const int tile = first + rank, st = round & 1;
     const int t0 = tile * kTile + warp * S;
-    bool rs_now[S];
+    cp_async_wait_all();
+    __syncthreads();  // the tile has landed; the other buffer is no longer read
+    if (tile + csize < tiles) load(tile + csize, st ^ 1);
+    cp_async_commit();
+    float2 m[S], u[S];
+    bool drop[S];
+    if (tile < tiles) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) rs_now[s] = kReset && rs[s];
-    float2 a[S], u[S];
+      for (int s = 0; s < S; ++s) {
+        const int row = warp * S + s;
+        float2 q;
+        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]))), m[s], q);
+        const float2 v =
+            mul2(sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane])), unpack2(&sm.raw[st][0][row][2 * lane]));
+        drop[s] = kReset && t0 + s < p.seq && rst[t0 + s] != 0;
+        u[s] = drop[s] ? v : mul2(mul2(q, inv_sqrt2(q)), v);
+      }
+    }
+    if (t0 + S > p.seq) {  // steps past the end keep the state
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (t0 + s >= p.seq) {
+          m[s] = u[s] = bc2(0.f);
+          drop[s] = false;
+        }
+    }
     float2 M = bc2(0.f), E = bc2(0.f);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      float2 m, q;
-      decay2(mul2(rate, sigmoid2(rr[s].get())), m, q);
-      const float2 v = mul2(sigmoid2(ir[s].get()), xr[s].get());
-      u[s] = mul2(mul2(q, inv_sqrt2(q)), v);
-      if (t0 + s >= p.seq) {  // past the end: the state is kept
-        m = bc2(0.f);
-        u[s] = bc2(0.f);
-      }
-      a[s] = add2(m, bc2(1.f));
-      if (kReset && rs_now[s]) {
-        a[s] = bc2(0.f);
-        u[s] = v;
-        E = v;
+      if (kReset && drop[s]) {
+        E = u[s];
         M = bc2(-1.f);
       } else {
-        E = fma2(a[s], E, u[s]);
-        M = join_decay(M, m);
+        E = fma2(add2(m[s], bc2(1.f)), E, u[s]);
+        M = join_decay(M, m[s]);
       }
     }
-    seg[buf][warp][lane] = make_float4(M.x, M.y, E.x, E.y);
-    // the next tile's rows are on their way while this one is joined and stored
-    if (first + csize < tiles) load(tile + csize);
+    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     __syncthreads();
-    // (PM, PE): the runs before this warp's; (TM, TE): the whole tile
-    float2 PM = bc2(0.f), PE = bc2(0.f), TM = bc2(0.f), TE = bc2(0.f);
+    if (tid < kChan) {
+      float h = carry;
+      if (csize > 1) {
+        float tm = 0.f, te = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w == warp) {
-        PM = TM;
-        PE = TE;
+        for (int w = 0; w < W; ++w) {
+          const float2 g = sm.run[w][tid];
+          te = apply<kReset>(g.x, g.y, te);
+          tm = join_decay(tm, g.x);
+        }
+        if (alive)
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, tm, te, p.status);
+        for (int k = 0; k < csize; ++k) {
+          if (k == rank) h = carry;
+          const float2 g = sm.ex.sum[st][k][tid];
+          carry = apply<kReset>(g.x, g.y, carry);
+        }
       }
-      const float4 g = seg[buf][w][lane];
-      const float2 gm = make_float2(g.x, g.y);
-      TE = apply<kReset>(gm, make_float2(g.z, g.w), TE);
-      TM = join_decay(TM, gm);
-    }
-    float2 h = carry;
-    if (csize > 1) {
-      if (warp < csize)
-        for (int to = warp; to < csize; to += W)
-          *cluster.map_shared_rank(&sum[buf][rank][lane], to) =
-              make_float4(TM.x, TM.y, TE.x, TE.y);
-      cluster.sync();
-      for (int k = 0; k < csize; ++k) {
-        if (k == rank) h = carry;
-        const float4 g = sum[buf][k][lane];
-        carry = apply<kReset>(make_float2(g.x, g.y), make_float2(g.z, g.w), carry);
+      if (p.ckpt != nullptr && jok && tile < tiles)
+        p.ckpt[(int64_t(b) * tiles + tile) * p.channels + jc] = h;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        sm.start[w][tid] = h;
+        const float2 g = sm.run[w][tid];
+        h = apply<kReset>(g.x, g.y, h);
       }
-    } else {
-      carry = apply<kReset>(TM, TE, carry);
+      if (csize == 1) carry = h;
     }
-    if (p.ckpt != nullptr && warp == 0 && tile < tiles)
-      store_f2(p.ckpt + (int64_t(b) * tiles + tile) * p.channels, h, ln);
-    h = apply<kReset>(PM, PE, h);
+    __syncthreads();
+    float2 h = *reinterpret_cast<const float2*>(&sm.start[warp][2 * lane]);
+    T* yt = y + int64_t(t0) * p.channels;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      h = kReset && rs_now[s] ? u[s] : fma2(a[s], h, u[s]);
-      const int t = t0 + s;
-      if (t < p.seq && ln.ok0)
-        Pair<T, kVec>::store(y + int64_t(t) * p.channels, h, ln.step, ln.ok0, ln.ok1);
+      h = kReset && drop[s] ? u[s] : fma2(add2(m[s], bc2(1.f)), h, u[s]);
+      if (t0 + s < p.seq) store2<kVec>(yt + int64_t(s) * p.channels, h, ok0, ok1);
     }
   }
-  if (p.hT != nullptr && rank == 0 && warp == 0)
-    store_f2(p.hT + int64_t(b) * p.channels, carry, ln);
+  if (p.hT != nullptr && rank == 0 && jok) p.hT[int64_t(b) * p.channels + jc] = carry;
+  if (csize > 1) cluster.sync();  // no CTA leaves while another may still write to it
 }
 
 // ------------------------------------------------------------------ backward
 
 constexpr int kBwdWarps = 16;
 
-template <typename T, bool kVec, bool kReset>
-__global__ void __launch_bounds__(kBwdWarps * 32)
+template <typename T>
+struct BwdSmem {
+  T raw[2][4][kTile][kChan];          // x, r, i, dy of this tile and the one before it
+  float2 run[kBwdWarps][kChan];       // (M, E) of each warp's run
+  float back[kBwdWarps][kChan];       // G of each run: c before it = A c after it + G
+  float start[kBwdWarps][kChan];      // state before each run
+  float after[kBwdWarps][kChan];      // c after each run
+  Exchange<kMaxCluster<T>> ex;
+};
+
+template <typename T, int kBytes, bool kVec, bool kReset>
+__global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
     gated_scan_bwd_kernel(const BwdArgs p) {
-  constexpr int W = kBwdWarps, S = kTile / W;
-  __shared__ float4 segf[2][W][32];  // (A0, A1, E0, E1) of each run
-  __shared__ float2 segb[2][W][32];  // G of each run: c_out = A c_in + G
-  __shared__ float4 sum[2][kMaxCluster][32];
-  __shared__ float2 red[W][32];
+  constexpr int W = kBwdWarps, S = kTile / W, kThreads = W * 32;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  BwdSmem<T>& sm = *reinterpret_cast<BwdSmem<T>*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int unit = int(blockIdx.x) / csize;
   const int b = unit / p.chan_tiles;
-  const Lane ln = lane_of<kVec>(unit - b * p.chan_tiles, p.channels);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = (unit - b * p.chan_tiles) * kChan;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int c = c0 + 2 * lane;
+  const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
   const int tiles = (p.seq + kTile - 1) / kTile;
   const int64_t row0 = int64_t(b) * p.seq;
-  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + ln.c;
-  const T* r = static_cast<const T*>(p.r) + row0 * p.rs + ln.c;
-  const T* iv = static_cast<const T*>(p.i) + row0 * p.is + ln.c;
-  const T* dy = static_cast<const T*>(p.dy) + (p.dy ? row0 * p.dys + ln.c : 0);
-  const int64_t out0 = row0 * p.channels + ln.c;
+  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + c0;
+  const T* r = static_cast<const T*>(p.r) + row0 * p.rs + c0;
+  const T* iv = static_cast<const T*>(p.i) + row0 * p.is + c0;
+  const T* dy = p.dy ? static_cast<const T*>(p.dy) + row0 * p.dys + c0 : nullptr;
+  const int64_t out0 = row0 * p.channels + c;
   const uint8_t* rst = kReset ? p.reset + row0 : nullptr;
-  const float2 lam = load_f2(p.lambda, ln);
+  const float2 lam = load_f2(p.lambda, c, ok0, ok1);
   const float2 rate = make_float2(p.sharpness * softplus_acc(lam.x), p.sharpness * softplus_acc(lam.y));
-  float2 carry = load_f2(p.dhT ? p.dhT + int64_t(b) * p.channels : nullptr, ln);
+  // threads 0 .. 63 join the states, 64 .. 127 the gradients, one channel each
+  const int jch = tid & (kChan - 1), jc = c0 + jch;
+  const bool jok = tid < 2 * kChan && jc < p.channels;
+  float carry = jok && p.dhT ? p.dhT[int64_t(b) * p.channels + jc] : 0.f;
   float2 dlam = bc2(0.f);
 
-  Pair<T, kVec> xr[S], rr[S], ir[S], gr[S];
-  bool rs[S];
-  float2 start;
-  auto load = [&](int tile) {
-    const int t0 = tile * kTile + warp * S;
-    start = bc2(0.f);
-    if (tile >= 0)
-      start = load_f2(p.ckpt + (int64_t(b) * tiles + tile) * p.channels, ln);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int t = t0 + s;
-      const bool in = t >= 0 && t < p.seq;
-      if (kReset) rs[s] = in && rst[t] != 0;
-      if (in && ln.ok0) {
-        xr[s].load(x + t * p.xs, ln.step, ln.ok0, ln.ok1);
-        rr[s].load(r + t * p.rs, ln.step, ln.ok0, ln.ok1);
-        ir[s].load(iv + t * p.is, ln.step, ln.ok0, ln.ok1);
-        if (p.dy != nullptr) gr[s].load(dy + t * p.dys, ln.step, ln.ok0, ln.ok1);
-        else gr[s] = Pair<T, kVec>{};
-      } else {
-        xr[s] = rr[s] = ir[s] = gr[s] = Pair<T, kVec>{};
-      }
-    }
+  auto load = [&](int tile, int st) {
+    const int64_t t0 = int64_t(tile) * kTile;
+    const int rows = p.seq - int(t0), cols = p.channels - c0;
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][0][0][0], x + t0 * p.xs, p.xs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][1][0][0], r + t0 * p.rs, p.rs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[st][2][0][0], iv + t0 * p.is, p.is, rows, cols);
+    if (dy != nullptr)
+      copy_tile<T, kBytes, kThreads>(&sm.raw[st][3][0][0], dy + t0 * p.dys, p.dys, rows, cols);
   };
+  if (dy == nullptr)
+    for (int k = tid; k < 2 * kTile * kChan; k += kThreads)
+      sm.raw[k / (kTile * kChan)][3][0][k % (kTile * kChan)] = T(0.f);
 
+  if (csize > 1) exchange_init(&sm.ex);
   // the cluster's tiles are taken from the end: rank 0 the last of each group
-  load(tiles - 1 - rank);
-  if (csize > 1) cluster.sync();  // every CTA has begun before its shared memory is written
-  int buf = 0;
-  for (int done = 0; done < tiles; done += csize, buf ^= 1) {
-    const int tile = tiles - 1 - done - rank;  // below 0: an empty tile
+  if (rank < tiles) load(tiles - 1 - rank, 0);
+  cp_async_commit();
+  if (csize > 1) cluster.sync();  // every CTA's mbarriers are ready before they are written
+  bool alive = true;
+  int round = 0;
+  for (int done = 0; done < tiles; done += csize, ++round) {
+    const int tile = tiles - 1 - done - rank, st = round & 1;  // below 0: an empty tile
     const int t0 = tile * kTile + warp * S;
-    float2 a[S], sr[S], si[S], xv[S], ib[S], q[S], g[S];
+    float h_tile = 0.f;
+    if (jok && tid < kChan && tile >= 0)
+      h_tile = p.ckpt[(int64_t(b) * tiles + tile) * p.channels + jc];
+    cp_async_wait_all();
+    __syncthreads();  // the tile has landed; the other buffer is no longer read
+    if (tile - csize >= 0) load(tile - csize, st ^ 1);
+    cp_async_commit();
+    const bool here = tile >= 0;
+    float2 m[S], sr[S], si[S];
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f), G = bc2(0.f);
-    const float2 h_tile = start;
+    if (here) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      sr[s] = sigmoid2(rr[s].get());
-      si[s] = sigmoid2(ir[s].get());
-      xv[s] = xr[s].get();
-      g[s] = gr[s].get();
-      float2 m;
-      decay2(mul2(rate, sr[s]), m, q[s]);
-      ib[s] = inv_sqrt2(q[s]);
-      drop[s] = kReset && rs[s];
-      const int t = t0 + s;
-      if (t < 0 || t >= p.seq) m = bc2(0.f);  // nothing there: c passes through (g is 0)
-      a[s] = add2(m, bc2(1.f));
-      const float2 v = mul2(si[s], xv[s]);
-      if (drop[s]) {
-        a[s] = bc2(0.f);
-        E = v;
-        M = bc2(-1.f);
-      } else {
-        E = fma2(a[s], E, mul2(mul2(q[s], ib[s]), v));
-        M = join_decay(M, m);
+      for (int s = 0; s < S; ++s) {
+        const int row = warp * S + s;
+        float2 q;
+        sr[s] = sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]));
+        si[s] = sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane]));
+        decay2(mul2(rate, sr[s]), m[s], q);
+        drop[s] = kReset && t0 + s < p.seq && rst[t0 + s] != 0;
+        const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][row][2 * lane]));
+        const float2 u = drop[s] ? v : mul2(mul2(q, inv_sqrt2(q)), v);
+        if (t0 + s >= p.seq) m[s] = bc2(0.f);  // past the end (x and dy are 0 there)
+        if (kReset && drop[s]) {
+          E = u;
+          M = bc2(-1.f);
+        } else {
+          E = fma2(add2(m[s], bc2(1.f)), E, u);
+          M = join_decay(M, m[s]);
+        }
+      }
+#pragma unroll
+      for (int s = S - 1; s >= 0; --s) {
+        const float2 g = add2(unpack2(&sm.raw[st][3][warp * S + s][2 * lane]), G);
+        G = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), g);
       }
     }
-#pragma unroll
-    for (int s = S - 1; s >= 0; --s) G = drop[s] ? bc2(0.f) : mul2(a[s], add2(g[s], G));
-    segf[buf][warp][lane] = make_float4(M.x, M.y, E.x, E.y);
-    segb[buf][warp][lane] = G;
-    if (done + csize < tiles) load(tile - csize);
+    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
+    *reinterpret_cast<float2*>(&sm.back[warp][2 * lane]) = G;
     __syncthreads();
-    float2 h = h_tile, PM = bc2(0.f), PG = bc2(0.f), TM = bc2(0.f), TG = bc2(0.f);
+    if (tid < kChan) {
+      float h = h_tile;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w < warp) {
-        const float4 f = segf[buf][w][lane];
-        h = apply<kReset>(make_float2(f.x, f.y), make_float2(f.z, f.w), h);
+      for (int w = 0; w < W; ++w) {
+        sm.start[w][jch] = h;
+        const float2 g = sm.run[w][jch];
+        h = apply<kReset>(g.x, g.y, h);
       }
-    }
+    } else if (tid < 2 * kChan) {
+      float cc = carry;
+      if (csize > 1) {
+        float tm = 0.f, tg = 0.f;
 #pragma unroll
-    for (int w = W - 1; w >= 0; --w) {
-      if (w == warp) {
-        PM = TM;
-        PG = TG;
+        for (int w = W - 1; w >= 0; --w) {
+          const float fm = sm.run[w][jch].x;
+          tg = apply<kReset>(fm, sm.back[w][jch], tg);
+          tm = join_decay(tm, fm);
+        }
+        if (alive)
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, tm, tg, p.status);
+        for (int k = 0; k < csize; ++k) {
+          if (k == rank) cc = carry;
+          const float2 g = sm.ex.sum[st][k][jch];
+          carry = apply<kReset>(g.x, g.y, carry);
+        }
       }
-      const float4 f = segf[buf][w][lane];
-      const float2 fm = make_float2(f.x, f.y);
-      TG = apply<kReset>(fm, segb[buf][w][lane], TG);
-      TM = join_decay(TM, fm);
-    }
-    float2 c = carry;
-    if (csize > 1) {
-      if (warp < csize)
-        *cluster.map_shared_rank(&sum[buf][rank][lane], warp) = make_float4(TM.x, TM.y, TG.x, TG.y);
-      cluster.sync();
-      for (int k = 0; k < csize; ++k) {
-        if (k == rank) c = carry;
-        const float4 f = sum[buf][k][lane];
-        carry = apply<kReset>(make_float2(f.x, f.y), make_float2(f.z, f.w), carry);
+#pragma unroll
+      for (int w = W - 1; w >= 0; --w) {
+        sm.after[w][jch] = cc;
+        cc = apply<kReset>(sm.run[w][jch].x, sm.back[w][jch], cc);
       }
-    } else {
-      carry = apply<kReset>(TM, TG, carry);
+      if (csize == 1) carry = cc;
     }
-    c = apply<kReset>(PM, PG, c);
-    // h[t-1] of each step forwards, then the gradients backwards
-    float2 hp[S];
+    __syncthreads();
+    if (here) {
+      // h[t-1] of each step forwards, then the gradients backwards
+      float2 h = *reinterpret_cast<const float2*>(&sm.start[warp][2 * lane]);
+      float2 cc = *reinterpret_cast<const float2*>(&sm.after[warp][2 * lane]);
+      float2 hp[S], ib[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      hp[s] = h;
-      const float2 v = mul2(si[s], xv[s]);
-      h = drop[s] ? v : fma2(a[s], h, mul2(mul2(q[s], ib[s]), v));
-    }
+      for (int s = 0; s < S; ++s) {
+        hp[s] = h;
+        const float2 q = mul2(neg2(m[s]), add2(m[s], bc2(2.f)));
+        ib[s] = inv_sqrt2(q);
+        const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][warp * S + s][2 * lane]));
+        h = kReset && drop[s] ? v : fma2(add2(m[s], bc2(1.f)), h, mul2(mul2(q, ib[s]), v));
+      }
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
-      const int t = t0 + s;
-      const float2 gs = add2(g[s], c);
-      c = drop[s] ? bc2(0.f) : mul2(a[s], gs);
-      const float2 beta = drop[s] ? bc2(1.f) : mul2(q[s], ib[s]);
-      const float2 gb = mul2(gs, beta);
-      const float2 dx = mul2(gb, si[s]);
-      const float2 di = mul2(mul2(dx, xv[s]), fma2(neg2(si[s]), bc2(1.f), bc2(1.f)));
-      // dL = g (a^2 / beta s(i) x - a h[t-1])
-      const float2 slope = mul2(mul2(a[s], ib[s]), mul2(si[s], xv[s]));
-      float2 dl = mul2(c, add2(slope, neg2(hp[s])));
-      if (drop[s] || t < 0 || t >= p.seq) dl = bc2(0.f);
-      const float2 ds = mul2(dl, sr[s]);
-      const float2 dr = mul2(mul2(ds, rate), fma2(neg2(sr[s]), bc2(1.f), bc2(1.f)));
-      dlam = add2(dlam, ds);
-      if (t >= 0 && t < p.seq && ln.ok0) {
-        const int64_t o = out0 + int64_t(t) * p.channels;
-        Pair<T, kVec>::store(static_cast<T*>(p.dx) + o, dx, ln.step, ln.ok0, ln.ok1);
-        Pair<T, kVec>::store(static_cast<T*>(p.dr) + o, dr, ln.step, ln.ok0, ln.ok1);
-        Pair<T, kVec>::store(static_cast<T*>(p.di) + o, di, ln.step, ln.ok0, ln.ok1);
+      for (int s = S - 1; s >= 0; --s) {
+        const int row = warp * S + s;
+        const float2 xv = unpack2(&sm.raw[st][0][row][2 * lane]);
+        const float2 gs = add2(unpack2(&sm.raw[st][3][row][2 * lane]), cc);
+        const float2 a = add2(m[s], bc2(1.f));
+        const float2 q = mul2(neg2(m[s]), add2(m[s], bc2(2.f)));
+        cc = kReset && drop[s] ? bc2(0.f) : mul2(a, gs);
+        const float2 gb = kReset && drop[s] ? gs : mul2(gs, mul2(q, ib[s]));
+        const float2 dx = mul2(gb, si[s]);
+        const float2 di = mul2(mul2(dx, xv), add2(bc2(1.f), neg2(si[s])));
+        // dL = g (a^2 / beta s(i) x - a h[t-1]) = c (a / beta s(i) x - h[t-1])
+        const float2 slope = mul2(mul2(a, ib[s]), mul2(si[s], xv));
+        float2 ds = mul2(mul2(cc, add2(slope, neg2(hp[s]))), sr[s]);
+        if (kReset && drop[s]) ds = bc2(0.f);
+        const float2 dr = mul2(mul2(ds, rate), add2(bc2(1.f), neg2(sr[s])));
+        if (t0 + s < p.seq) {
+          dlam = add2(dlam, ds);
+          const int64_t o = out0 + int64_t(t0 + s) * p.channels;
+          store2<kVec>(static_cast<T*>(p.dx) + o, dx, ok0, ok1);
+          store2<kVec>(static_cast<T*>(p.dr) + o, dr, ok0, ok1);
+          store2<kVec>(static_cast<T*>(p.di) + o, di, ok0, ok1);
+        }
       }
     }
   }
-  if (p.dh0 != nullptr && rank == 0 && warp == 0)
-    store_f2(p.dh0 + int64_t(b) * p.channels, carry, ln);
+  if (p.dh0 != nullptr && rank == 0 && jok && tid >= kChan) p.dh0[int64_t(b) * p.channels + jc] = carry;
+  __syncthreads();
+  float2(*red)[32] = reinterpret_cast<float2(*)[32]>(&sm.run[0][0]);
   red[warp][lane] = dlam;
   __syncthreads();
   if (warp == 0) {
     float2 t = red[0][lane];
     for (int w = 1; w < W; ++w) t = add2(t, red[w][lane]);
-    store_f2(p.part + (int64_t(b) * csize + rank) * p.channels, t, ln);
+    float* q = p.part + (int64_t(b) * csize + rank) * p.channels + c;
+    if (ok0) q[0] = t.x;
+    if (ok1) q[1] = t.y;
   }
+  if (csize > 1) cluster.sync();  // no CTA leaves while another may still write to it
 }
 
 // dLambda[ch] = c s(Lambda) sum over rows of part, in a fixed order.
@@ -562,6 +654,7 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------ one token
 
+// A thread takes two adjacent channels of one sequence.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(128)
     gated_step_kernel(const T* __restrict__ x, const T* __restrict__ r, const T* __restrict__ i,
@@ -571,25 +664,24 @@ __global__ void __launch_bounds__(128)
   const int64_t n = int64_t(blockIdx.x) * 128 + threadIdx.x;
   const int64_t b = n / pairs;
   if (b >= batch) return;
-  Lane ln;
-  ln.step = 1;
-  ln.c = int(n - b * pairs) * 2;
-  ln.ok0 = true;
-  ln.ok1 = ln.c + 1 < channels;
-  Pair<T, kVec> xr, rr, ir;
-  xr.load(x + b * xs + ln.c, 1, true, ln.ok1);
-  rr.load(r + b * rs + ln.c, 1, true, ln.ok1);
-  ir.load(i + b * is + ln.c, 1, true, ln.ok1);
-  float* hb = h + b * channels;
-  const float2 h0 = load_f2(hb, ln);
-  const float2 lam = load_f2(lambda, ln);
+  const int c = int(n - b * pairs) * 2;
+  const bool ok1 = c + 1 < channels;
+  auto load = [&](const T* p) {
+    if constexpr (kVec) return unpack2(p);
+    else return make_float2(to_f(p[0]), ok1 ? to_f(p[1]) : 0.f);
+  };
+  const float2 xv = load(x + b * xs + c), rv = load(r + b * rs + c), iv = load(i + b * is + c);
+  float* hb = h + b * channels + c;
+  const float2 h0 = make_float2(hb[0], ok1 ? hb[1] : 0.f);
+  const float2 lam = load_f2(lambda, c, true, ok1);
   const float2 rate = make_float2(sharpness * softplus_acc(lam.x), sharpness * softplus_acc(lam.y));
   float2 m, q;
-  decay2(mul2(rate, sigmoid2(rr.get())), m, q);
-  const float2 u = mul2(mul2(q, inv_sqrt2(q)), mul2(sigmoid2(ir.get()), xr.get()));
+  decay2(mul2(rate, sigmoid2(rv)), m, q);
+  const float2 u = mul2(mul2(q, inv_sqrt2(q)), mul2(sigmoid2(iv), xv));
   const float2 hn = fma2(add2(m, bc2(1.f)), h0, u);
-  store_f2(hb, hn, ln);
-  Pair<T, kVec>::store(y + b * channels + ln.c, hn, 1, true, ln.ok1);
+  hb[0] = hn.x;
+  if (ok1) hb[1] = hn.y;
+  store2<kVec>(y + b * channels + c, hn, true, ok1);
 }
 
 // ----------------------------------------------------------------------- host
@@ -601,92 +693,93 @@ struct Fit {
   std::atomic<int> clusters[5];
 };
 
+cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, int64_t grid, int threads, size_t smem,
+                                  int c, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  at->id = cudaLaunchAttributeClusterDimension;
+  at->val.clusterDim.x = unsigned(c);
+  at->val.clusterDim.y = at->val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
 template <typename K>
-void ask_fit(K kernel, int threads, Fit& fit) {
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (most > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   for (int k = 0; k < 5; ++k) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1u << k);
-    cfg.blockDim = dim3(unsigned(threads));
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 1u << k;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    cudaLaunchAttribute at;
+    const cudaLaunchConfig_t cfg = cluster_config(&at, 1 << k, threads, smem, 1 << k, nullptr);
+    if ((1 << k) > most || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
     cudaGetLastError();
     fit.clusters[k].store(n);
   }
   fit.known.store(1);
 }
 
-// Cluster size: the CTAs of a cluster take consecutive tiles of one sequence. The
-// one that needs the fewest rounds of a tile, by how many clusters fit at once; no
-// more CTAs than tiles.
-template <auto kernel>
-int cluster_size(int threads, int64_t units, int tiles) {
+// Launches `units` clusters, one for each 64 channels of a sequence. The CTAs of a
+// cluster take consecutive tiles; of the sizes that fit (no more CTAs than tiles) it
+// is the one that needs the fewest rounds of a tile. *size: the size taken.
+template <auto kernel, typename A>
+int launch_clusters(const char* what, const A& args, int threads, size_t smem, int most,
+                    int64_t units, int tiles, cudaStream_t st, int* size) {
   static Fit fits[64];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  cudaError_t e = cudaGetDevice(&dev);
+  MQC_REQUIRE(e == cudaSuccess && dev >= 0 && dev < 64, MQC_ERR_CUDA, "%s: no device", what);
   Fit& fit = fits[dev];
-  if (!fit.known.load()) ask_fit(kernel, threads, fit);
-  int best = 1;
+  if (!fit.known.load()) ask_fit(kernel, threads, smem, most, fit);
+  int c = 0;
   int64_t least = INT64_MAX;
-  for (int k = 0; k < 5; ++k) {
-    const int c = 1 << k, n = fit.clusters[k].load();
-    if (c > tiles || n <= 0) break;
-    const int64_t rounds = ((units + n - 1) / n) * ((tiles + c - 1) / c);
+  for (int k = 0; k < 5 && (c == 0 || (1 << k) <= tiles); ++k) {
+    const int n = fit.clusters[k].load();
+    if (n <= 0) continue;
+    const int64_t rounds = ((units + n - 1) / n) * ((tiles + (1 << k) - 1) >> k);
     if (rounds < least) {
       least = rounds;
-      best = c;
+      c = 1 << k;
     }
   }
-  return best;
-}
-
-template <typename K, typename A>
-int launch_clusters(const char* what, K kernel, const A& args, int threads, int64_t units, int c,
-                    cudaStream_t st) {
+  MQC_REQUIRE(c > 0, MQC_ERR_CUDA, "%s: the kernel does not fit the device", what);
   MQC_REQUIRE(units * c <= 0x7fffffffll, MQC_ERR_UNSUPPORTED, "%s: too many channel tiles", what);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(units * c));
-  cfg.blockDim = dim3(unsigned(threads));
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = unsigned(c);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  cudaLaunchAttribute at;
+  const cudaLaunchConfig_t cfg = cluster_config(&at, units * c, threads, smem, c, st);
+  e = cudaLaunchKernelEx(&cfg, kernel, args);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(MQC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   }
+  *size = c;
   return check_launch(what);
 }
 
-template <typename T, bool kVec, bool kReset>
+template <typename T, int kBytes, bool kVec, bool kReset>
 int run_fwd(const FwdArgs& f, cudaStream_t st) {
-  constexpr auto kernel = &gated_scan_fwd_kernel<T, kVec, kReset>;
-  const int64_t units = int64_t(f.batch) * f.chan_tiles;
-  const int c = cluster_size<kernel>(kFwdWarps * 32, units, (f.seq + kTile - 1) / kTile);
-  return launch_clusters("mqc_gated_scan_fwd", kernel, f, kFwdWarps * 32, units, c, st);
+  int c;
+  return launch_clusters<&gated_scan_fwd_kernel<T, kBytes, kVec, kReset>>(
+      "mqc_gated_scan_fwd", f, kFwdWarps * 32, sizeof(FwdSmem<T>), kMaxCluster<T>,
+      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, st, &c);
 }
 
-template <typename T, bool kVec, bool kReset>
+template <typename T, int kBytes, bool kVec, bool kReset>
 int run_bwd(const BwdArgs& f, float* dlambda, cudaStream_t st) {
-  constexpr auto kernel = &gated_scan_bwd_kernel<T, kVec, kReset>;
-  const int64_t units = int64_t(f.batch) * f.chan_tiles;
-  const int c = cluster_size<kernel>(kBwdWarps * 32, units, (f.seq + kTile - 1) / kTile);
-  if (int rc = launch_clusters("mqc_gated_scan_bwd", kernel, f, kBwdWarps * 32, units, c, st))
+  int c = 0;
+  if (int rc = launch_clusters<&gated_scan_bwd_kernel<T, kBytes, kVec, kReset>>(
+          "mqc_gated_scan_bwd", f, kBwdWarps * 32, sizeof(BwdSmem<T>), kMaxCluster<T>,
+          int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, st, &c))
     return rc;
   gated_scan_dlambda_kernel<<<(f.channels + 31) / 32, 256, 0, st>>>(
       f.part, f.lambda, dlambda, f.batch * c, f.channels, f.sharpness);
   return check_launch("mqc_gated_scan_bwd (dLambda)");
 }
+
+constexpr int kLargestCluster = 16;
 
 int check_sizes(const char* what, const mqc_gated_scan_args* a) {
   MQC_REQUIRE(a != nullptr, MQC_ERR_INVALID_VALUE, "%s: args is NULL", what);
@@ -694,8 +787,8 @@ int check_sizes(const char* what, const mqc_gated_scan_args* a) {
   MQC_REQUIRE(a->batch >= 0 && a->seq_len >= 0 && a->channels >= 0, MQC_ERR_INVALID_VALUE,
               "%s: batch %lld, seq_len %lld, channels %lld", what, (long long)a->batch,
               (long long)a->seq_len, (long long)a->channels);
-  MQC_REQUIRE(a->seq_len <= 0x7fffffff - 2 * kMaxCluster * kTile && a->channels <= 0x7fffffff - kChan &&
-                  a->batch <= 0x7fffffff / kMaxCluster,
+  MQC_REQUIRE(a->seq_len <= 0x7fffffff - 2 * kLargestCluster * kTile && a->channels <= 0x7fffffff - kChan &&
+                  a->batch <= 0x7fffffff / kLargestCluster,
               MQC_ERR_UNSUPPORTED, "%s: a size above 2^31", what);
   MQC_REQUIRE(a->sharpness > 0.f, MQC_ERR_INVALID_VALUE, "%s: sharpness %g", what,
               double(a->sharpness));
@@ -713,15 +806,26 @@ int check_inputs(const char* what, const mqc_gated_scan_args* a) {
   return MQC_OK;
 }
 
-// Adjacent channel pairs can move as one word: even widths and strides, aligned bases.
-bool pairs_ok(int64_t channels, uintptr_t es, std::initializer_list<const void*> ptrs,
-              std::initializer_list<int64_t> strides) {
-  if (channels % 2) return false;
+// Whether `group` adjacent channels can move as one word: strides and bases are
+// multiples of it.
+bool groups_ok(int64_t group, uintptr_t es, std::initializer_list<const void*> ptrs,
+               std::initializer_list<int64_t> strides) {
   for (const void* q : ptrs)
-    if (!aligned(q, 2 * es)) return false;
+    if (!aligned(q, group * es)) return false;
   for (int64_t s : strides)
-    if (s % 2) return false;
+    if (s % group) return false;
   return true;
+}
+
+// What a copy into shared memory moves at once, by alignment: 16 bytes, 4, or (bf16
+// of odd stride or base) 2. Pairs of channels are stored as one word with the first
+// two of bf16 and the first of fp32.
+int copy_bytes(int64_t channels, uintptr_t es, std::initializer_list<const void*> in,
+               std::initializer_list<const void*> out, std::initializer_list<int64_t> strides) {
+  const bool pairs = channels % 2 == 0 && groups_ok(2, es, out, {});
+  if (pairs && groups_ok(16 / es, es, in, strides)) return 16;
+  if (es == 4 || (pairs && groups_ok(2, es, in, strides))) return 4;
+  return 2;
 }
 
 }  // namespace
@@ -752,20 +856,23 @@ int mqc_gated_scan_fwd(const mqc_gated_scan_args* a, void* stream) {
   FwdArgs f = {a->x, a->r, a->i, a->x_row, a->r_row, a->i_row,
                static_cast<const float*>(a->lambda_), static_cast<const float*>(a->h0),
                static_cast<const uint8_t*>(a->reset), a->y, static_cast<float*>(a->hT),
-               static_cast<float*>(a->ckpt), int(a->batch), int(a->seq_len), int(a->channels),
+               static_cast<float*>(a->ckpt), static_cast<int*>(a->status), int(a->batch),
+               int(a->seq_len), int(a->channels),
                int((a->channels + kChan - 1) / kChan), a->sharpness};
-  const bool vec = pairs_ok(a->channels, es, {a->x, a->r, a->i, a->y}, {a->x_row, a->r_row, a->i_row});
-  const bool rst = a->reset != nullptr, f32 = a->dtype == MQC_DTYPE_F32;
-#define MQC_RUN(T) \
-  (vec ? (rst ? run_fwd<T, true, true>(f, st) : run_fwd<T, true, false>(f, st)) \
-       : (rst ? run_fwd<T, false, true>(f, st) : run_fwd<T, false, false>(f, st)))
-  return f32 ? MQC_RUN(float) : MQC_RUN(__nv_bfloat16);
+  const int bytes = copy_bytes(a->channels, es, {a->x, a->r, a->i}, {a->y},
+                               {a->x_row, a->r_row, a->i_row});
+  const bool rst = a->reset != nullptr;
+#define MQC_RUN(...) (rst ? run_fwd<__VA_ARGS__, true>(f, st) : run_fwd<__VA_ARGS__, false>(f, st))
+  if (a->dtype == MQC_DTYPE_F32)
+    return bytes == 16 ? MQC_RUN(float, 16, true) : MQC_RUN(float, 4, false);
+  if (bytes == 16) return MQC_RUN(__nv_bfloat16, 16, true);
+  return bytes == 4 ? MQC_RUN(__nv_bfloat16, 4, true) : MQC_RUN(__nv_bfloat16, 2, false);
 #undef MQC_RUN
 }
 
 size_t mqc_gated_scan_bwd_workspace_size(int64_t batch, int64_t seq_len, int64_t channels) {
   if (batch <= 0 || seq_len <= 0 || channels <= 0) return 0;
-  return size_t(batch) * size_t(channels) * mqc::kMaxCluster * sizeof(float);
+  return size_t(batch) * size_t(channels) * mqc::kLargestCluster * sizeof(float);
 }
 
 int mqc_gated_scan_bwd(const mqc_gated_scan_args* a, void* workspace, size_t workspace_bytes,
@@ -804,17 +911,19 @@ int mqc_gated_scan_bwd(const mqc_gated_scan_args* a, void* workspace, size_t wor
   BwdArgs f = {a->x, a->r, a->i, a->dy, a->x_row, a->r_row, a->i_row, a->dy_row,
                static_cast<const float*>(a->lambda_), static_cast<const uint8_t*>(a->reset),
                static_cast<const float*>(a->ckpt), static_cast<const float*>(a->dhT), a->dx, a->dr,
-               a->di, static_cast<float*>(a->dh0), static_cast<float*>(workspace), int(a->batch),
-               int(a->seq_len), int(a->channels), int((a->channels + kChan - 1) / kChan),
+               a->di, static_cast<float*>(a->dh0), static_cast<float*>(workspace),
+               static_cast<int*>(a->status), int(a->batch), int(a->seq_len), int(a->channels), int((a->channels + kChan - 1) / kChan),
                a->sharpness};
   float* dl = static_cast<float*>(a->dlambda);
-  const bool vec = pairs_ok(a->channels, es, {a->x, a->r, a->i, a->dy, a->dx, a->dr, a->di},
-                            {a->x_row, a->r_row, a->i_row, a->dy ? a->dy_row : 0});
-  const bool rst = a->reset != nullptr, f32 = a->dtype == MQC_DTYPE_F32;
-#define MQC_RUN(T) \
-  (vec ? (rst ? run_bwd<T, true, true>(f, dl, st) : run_bwd<T, true, false>(f, dl, st)) \
-       : (rst ? run_bwd<T, false, true>(f, dl, st) : run_bwd<T, false, false>(f, dl, st)))
-  return f32 ? MQC_RUN(float) : MQC_RUN(__nv_bfloat16);
+  const int bytes = copy_bytes(a->channels, es, {a->x, a->r, a->i, a->dy}, {a->dx, a->dr, a->di},
+                               {a->x_row, a->r_row, a->i_row, a->dy ? a->dy_row : 0});
+  const bool rst = a->reset != nullptr;
+#define MQC_RUN(...) \
+  (rst ? run_bwd<__VA_ARGS__, true>(f, dl, st) : run_bwd<__VA_ARGS__, false>(f, dl, st))
+  if (a->dtype == MQC_DTYPE_F32)
+    return bytes == 16 ? MQC_RUN(float, 16, true) : MQC_RUN(float, 4, false);
+  if (bytes == 16) return MQC_RUN(__nv_bfloat16, 16, true);
+  return bytes == 4 ? MQC_RUN(__nv_bfloat16, 4, true) : MQC_RUN(__nv_bfloat16, 2, false);
 #undef MQC_RUN
 }
 
@@ -839,7 +948,7 @@ int mqc_gated_scan_step(const void* x, int64_t x_row, const void* r, int64_t r_r
   const int pairs = int((channels + 1) / 2);
   const int64_t blocks = (batch * pairs + 127) / 128;
   MQC_REQUIRE(blocks <= 0x7fffffffll, MQC_ERR_UNSUPPORTED, "mqc_gated_scan_step: too large");
-  const bool vec = pairs_ok(channels, es, {x, r, i, y}, {x_row, r_row, i_row});
+  const bool vec = channels % 2 == 0 && groups_ok(2, es, {x, r, i, y}, {x_row, r_row, i_row});
   cudaStream_t st = as_stream(stream);
 #define MQC_STEP(T, V)                                                                       \
   gated_step_kernel<T, V><<<unsigned(blocks), 128, 0, st>>>(                                 \

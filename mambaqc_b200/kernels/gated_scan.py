@@ -49,6 +49,7 @@ def _forward(x, r, i, lam, h0, reset, sharpness, want_state, keep):
     a.x_row, a.r_row, a.i_row = max(x_row, dm), max(r_row, dm), max(i_row, dm)
     a.lambda_, a.h0, a.reset = lam.data_ptr(), _lib.ptr(h0), _lib.ptr(reset)
     a.y, a.hT, a.ckpt = y.data_ptr(), _lib.ptr(hT), _lib.ptr(ckpt)
+    a.status = _lib.status_word(dev).data_ptr()
     _lib.call_on(dev, "mqc_gated_scan_fwd", ctypes.byref(a))
     return y, hT, (xs, rs, si, ckpt)
 
@@ -90,6 +91,7 @@ class _GatedScan(torch.autograd.Function):
         a.dy, a.dy_row, a.dhT = _lib.ptr(dys), max(dy_row, dm), _lib.ptr(dhT)
         a.dx, a.dr, a.di = dx.data_ptr(), dr.data_ptr(), di.data_ptr()
         a.dlambda, a.dh0 = dlam.data_ptr(), _lib.ptr(dh0)
+        a.status = _lib.status_word(dev).data_ptr()
         _lib.call_on(dev, "mqc_gated_scan_bwd", ctypes.byref(a), ws.data_ptr(), nbytes)
         return (dx, dr, di, dlam.to(lam_dtype), None if dh0 is None else dh0.to(h0_dtype),
                 None, None, None)
