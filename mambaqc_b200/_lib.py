@@ -278,14 +278,20 @@ def call(name: str, *args) -> None:
     check(getattr(lib, name)(*args), name)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device`` current and its current stream as the last argument."""
-    idx = device.index
-    if idx is None or idx == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+# the current stream's handle without building a torch.cuda.Stream (0.1 us against 2)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
+def call_on(idx: int, name: str, *args) -> None:
+    """``call`` with device ``idx`` current and its current stream as the last argument."""
+    if idx == torch.cuda.current_device():
+        rc = getattr(_lib or load(), name)(*args, _raw_stream(idx))
+        if rc != MQC_OK:
+            check(rc, name)
     else:
-        with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(idx):
+            call(name, *args, _raw_stream(idx))
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -25,6 +25,7 @@
 
 #include <atomic>
 #include <initializer_list>
+#include <type_traits>
 
 #include "mqc_common.cuh"
 #include "mqc_host.h"
@@ -65,13 +66,12 @@ __device__ __forceinline__ float rsqrt_a(float v) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-
-// minimum and maximum that keep a NaN
-__device__ __forceinline__ float min_nan(float a, float b) {
+__device__ __forceinline__ float sqrt_a(float v) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// maximum that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -79,27 +79,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kLeastNormal = 1.17549435e-38f;
 
-// 1 / (1 + 2^(-z log2 e)); the exponent is held at 126, where the result is 2^-126.
+// 1 / (1 + 2^(-z log2 e)); 0 where the power is infinite
 __device__ __forceinline__ float2 sigmoid2(float2 z) {
   const float2 e = mul2(z, bc2(-kLog2e));
-  const float2 d = add2(make_float2(ex2(min_nan(e.x, 126.f)), ex2(min_nan(e.y, 126.f))), bc2(1.f));
+  const float2 d = add2(make_float2(ex2(e.x), ex2(e.y)), bc2(1.f));
   return make_float2(rcp(d.x), rcp(d.y));
 }
 
 // exp(-l) - 1 for l >= 0: with -l = n ln 2 + f, |f| <= ln 2 / 2, it is
 // 2^n (e^f - 1) + (2^n - 1), e^f - 1 by its Taylor polynomial of degree 7
-// (remainder f^8 / 8!: below 2e-8 of f). Exact to the last place near l = 0, where
-// 1 - exp(-2 l) and the decay over many steps need it.
+// (remainder f^8 / 8!: below 2e-8 of f). Exact to the last place near l = 0 (n = 0),
+// where 1 - exp(-2 l) and the decay over many steps need it; for n < 0 the rounding of
+// n ln 2 adds 2e-8 n to f, less than 2^n / 4 of that to the result.
 __device__ __forceinline__ float2 expm1_neg2(float2 l) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
-  constexpr float kLn2Hi = 0.693145751953125f;  // 16 bits: n * hi is exact
-  constexpr float kLn2Lo = 1.42860682030941723e-6f;
   const float2 x = make_float2(max_nan(-l.x, -87.f), max_nan(-l.y, -87.f));
   const float2 t = fma2(x, bc2(kLog2e), bc2(kMagic));
   const float2 n = add2(t, bc2(-kMagic));
-  const float2 f = fma2(n, bc2(-kLn2Lo), fma2(n, bc2(-kLn2Hi), x));
+  const float2 f = fma2(n, bc2(-0.693147180559945309f), x);
   float2 p = fma2(f, bc2(1.f / 5040.f), bc2(1.f / 720.f));
   p = fma2(p, f, bc2(1.f / 120.f));
   p = fma2(p, f, bc2(1.f / 24.f));
@@ -139,11 +137,12 @@ __device__ __forceinline__ float apply(float M, float E, float s) {
   return kDrop && M == -1.f ? E : r;
 }
 
-// 1 / sqrt(q); 0 where q is 0 or subnormal (no decay to speak of: neither the
-// input's factor, 1e-19 at most, nor its slope counts)
+// sqrt(q), and 1 / sqrt(q) (1e19 at most: at q = 0 its product with q is 0, and what
+// else it multiplies is multiplied by L = 0 as well)
+__device__ __forceinline__ float2 sqrt2(float2 q) { return make_float2(sqrt_a(q.x), sqrt_a(q.y)); }
 __device__ __forceinline__ float2 inv_sqrt2(float2 q) {
-  return make_float2(q.x >= kLeastNormal ? rsqrt_a(q.x) : 0.f,
-                     q.y >= kLeastNormal ? rsqrt_a(q.y) : 0.f);
+  const float2 t = add2(q, bc2(1.17549435e-38f));
+  return make_float2(rsqrt_a(t.x), rsqrt_a(t.y));
 }
 
 // ------------------------------------------------------------------- memory
@@ -363,39 +362,35 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     __syncthreads();  // the tile has landed; the other buffer is no longer read
     if (tile + csize < tiles) load(tile + csize, st ^ 1);
     cp_async_commit();
-    float2 m[S], u[S];
+    float2 a[S], u[S];
     bool drop[S];
-    if (tile < tiles) {
+    float2 M = bc2(0.f), E = bc2(0.f);
+    // steps past the end keep the state; whole tiles do not look for it
+    auto reduce = [&](auto whole) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
-        float2 q;
-        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]))), m[s], q);
+        const bool in = decltype(whole)::value || t0 + s < p.seq;
+        float2 m, q;
+        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]))), m, q);
         const float2 v =
             mul2(sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane])), unpack2(&sm.raw[st][0][row][2 * lane]));
-        drop[s] = kReset && t0 + s < p.seq && rst[t0 + s] != 0;
-        u[s] = drop[s] ? v : mul2(mul2(q, inv_sqrt2(q)), v);
-      }
-    }
-    if (t0 + S > p.seq) {  // steps past the end keep the state
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (t0 + s >= p.seq) {
-          m[s] = u[s] = bc2(0.f);
-          drop[s] = false;
+        u[s] = mul2(sqrt2(q), v);
+        drop[s] = kReset && in && rst[t0 + s] != 0;
+        if (!in) m = u[s] = bc2(0.f);
+        a[s] = add2(m, bc2(1.f));
+        if (kReset && drop[s]) {
+          u[s] = E = v;
+          M = bc2(-1.f);
+        } else {
+          E = fma2(a[s], E, u[s]);
+          M = join_decay(M, m);
         }
-    }
-    float2 M = bc2(0.f), E = bc2(0.f);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (kReset && drop[s]) {
-        E = u[s];
-        M = bc2(-1.f);
-      } else {
-        E = fma2(add2(m[s], bc2(1.f)), E, u[s]);
-        M = join_decay(M, m[s]);
       }
-    }
+    };
+    const bool whole = (tile + 1) * kTile <= p.seq;
+    if (whole) reduce(std::true_type{});
+    else if (tile < tiles) reduce(std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     __syncthreads();
     if (tid < kChan) {
@@ -429,11 +424,16 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     __syncthreads();
     float2 h = *reinterpret_cast<const float2*>(&sm.start[warp][2 * lane]);
     T* yt = y + int64_t(t0) * p.channels;
+    auto write = [&](auto whole) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      h = kReset && drop[s] ? u[s] : fma2(add2(m[s], bc2(1.f)), h, u[s]);
-      if (t0 + s < p.seq) store2<kVec>(yt + int64_t(s) * p.channels, h, ok0, ok1);
-    }
+      for (int s = 0; s < S; ++s) {
+        h = kReset && drop[s] ? u[s] : fma2(a[s], h, u[s]);
+        if (decltype(whole)::value || t0 + s < p.seq) store2<kVec>(yt, h, ok0, ok1);
+        yt += p.channels;
+      }
+    };
+    if (whole) write(std::true_type{});
+    else if (tile < tiles) write(std::false_type{});
   }
   if (p.hT != nullptr && rank == 0 && jok) p.hT[int64_t(b) * p.channels + jc] = carry;
   if (csize > 1) cluster.sync();  // no CTA leaves while another may still write to it
@@ -454,7 +454,7 @@ struct BwdSmem {
 };
 
 template <typename T, int kBytes, bool kVec, bool kReset>
-__global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
+__global__ void __launch_bounds__(kBwdWarps * 32)
     gated_scan_bwd_kernel(const BwdArgs p) {
   constexpr int W = kBwdWarps, S = kTile / W, kThreads = W * 32;
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -513,27 +513,28 @@ __global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
     __syncthreads();  // the tile has landed; the other buffer is no longer read
     if (tile - csize >= 0) load(tile - csize, st ^ 1);
     cp_async_commit();
-    const bool here = tile >= 0;
-    float2 m[S], sr[S], si[S];
+    float2 m[S], sr[S], si[S], ib[S];
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f), G = bc2(0.f);
-    if (here) {
+    // steps past the end pass c on (x and dy are 0 there); whole tiles do not look for it
+    auto reduce = [&](auto whole) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
+        const bool in = decltype(whole)::value || t0 + s < p.seq;
         float2 q;
         sr[s] = sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]));
         si[s] = sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane]));
         decay2(mul2(rate, sr[s]), m[s], q);
-        drop[s] = kReset && t0 + s < p.seq && rst[t0 + s] != 0;
+        ib[s] = inv_sqrt2(q);
+        drop[s] = kReset && in && rst[t0 + s] != 0;
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][row][2 * lane]));
-        const float2 u = drop[s] ? v : mul2(mul2(q, inv_sqrt2(q)), v);
-        if (t0 + s >= p.seq) m[s] = bc2(0.f);  // past the end (x and dy are 0 there)
+        if (!in) m[s] = bc2(0.f);
         if (kReset && drop[s]) {
-          E = u;
+          E = v;
           M = bc2(-1.f);
         } else {
-          E = fma2(add2(m[s], bc2(1.f)), E, u);
+          E = fma2(add2(m[s], bc2(1.f)), E, mul2(mul2(q, ib[s]), v));
           M = join_decay(M, m[s]);
         }
       }
@@ -542,7 +543,10 @@ __global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
         const float2 g = add2(unpack2(&sm.raw[st][3][warp * S + s][2 * lane]), G);
         G = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), g);
       }
-    }
+    };
+    const bool here = tile >= 0, whole = here && (tile + 1) * kTile <= p.seq;
+    if (whole) reduce(std::true_type{});
+    else if (here) reduce(std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     *reinterpret_cast<float2*>(&sm.back[warp][2 * lane]) = G;
     __syncthreads();
@@ -580,36 +584,32 @@ __global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
       if (csize == 1) carry = cc;
     }
     __syncthreads();
-    if (here) {
-      // h[t-1] of each step forwards, then the gradients backwards
+    // h[t-1] of each step forwards, then the gradients backwards
+    auto write = [&](auto whole) {
       float2 h = *reinterpret_cast<const float2*>(&sm.start[warp][2 * lane]);
       float2 cc = *reinterpret_cast<const float2*>(&sm.after[warp][2 * lane]);
-      float2 hp[S], ib[S];
+      float2 term[S];  // a / beta s(i) x - h[t-1]: what c is multiplied by in dL
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        hp[s] = h;
-        const float2 q = mul2(neg2(m[s]), add2(m[s], bc2(2.f)));
-        ib[s] = inv_sqrt2(q);
+        const float2 a = add2(m[s], bc2(1.f));
+        const float2 beta = mul2(mul2(neg2(m[s]), add2(m[s], bc2(2.f))), ib[s]);
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][warp * S + s][2 * lane]));
-        h = kReset && drop[s] ? v : fma2(add2(m[s], bc2(1.f)), h, mul2(mul2(q, ib[s]), v));
+        term[s] = fma2(mul2(a, ib[s]), v, neg2(h));
+        h = kReset && drop[s] ? v : fma2(a, h, mul2(beta, v));
+        ib[s] = kReset && drop[s] ? bc2(1.f) : beta;  // beta from here on
       }
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         const int row = warp * S + s;
-        const float2 xv = unpack2(&sm.raw[st][0][row][2 * lane]);
         const float2 gs = add2(unpack2(&sm.raw[st][3][row][2 * lane]), cc);
-        const float2 a = add2(m[s], bc2(1.f));
-        const float2 q = mul2(neg2(m[s]), add2(m[s], bc2(2.f)));
-        cc = kReset && drop[s] ? bc2(0.f) : mul2(a, gs);
-        const float2 gb = kReset && drop[s] ? gs : mul2(gs, mul2(q, ib[s]));
-        const float2 dx = mul2(gb, si[s]);
-        const float2 di = mul2(mul2(dx, xv), add2(bc2(1.f), neg2(si[s])));
-        // dL = g (a^2 / beta s(i) x - a h[t-1]) = c (a / beta s(i) x - h[t-1])
-        const float2 slope = mul2(mul2(a, ib[s]), mul2(si[s], xv));
-        float2 ds = mul2(mul2(cc, add2(slope, neg2(hp[s]))), sr[s]);
+        cc = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), gs);
+        const float2 dx = mul2(mul2(gs, ib[s]), si[s]);
+        const float2 di = mul2(mul2(dx, unpack2(&sm.raw[st][0][row][2 * lane])),
+                               add2(bc2(1.f), neg2(si[s])));
+        float2 ds = mul2(mul2(cc, term[s]), sr[s]);
         if (kReset && drop[s]) ds = bc2(0.f);
         const float2 dr = mul2(mul2(ds, rate), add2(bc2(1.f), neg2(sr[s])));
-        if (t0 + s < p.seq) {
+        if (decltype(whole)::value || t0 + s < p.seq) {
           dlam = add2(dlam, ds);
           const int64_t o = out0 + int64_t(t0 + s) * p.channels;
           store2<kVec>(static_cast<T*>(p.dx) + o, dx, ok0, ok1);
@@ -617,7 +617,9 @@ __global__ void __launch_bounds__(kBwdWarps * 32, sizeof(T) == 2 ? 2 : 1)
           store2<kVec>(static_cast<T*>(p.di) + o, di, ok0, ok1);
         }
       }
-    }
+    };
+    if (whole) write(std::true_type{});
+    else if (here) write(std::false_type{});
   }
   if (p.dh0 != nullptr && rank == 0 && jok && tid >= kChan) p.dh0[int64_t(b) * p.channels + jc] = carry;
   __syncthreads();
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(128)
   const float2 rate = make_float2(sharpness * softplus_acc(lam.x), sharpness * softplus_acc(lam.y));
   float2 m, q;
   decay2(mul2(rate, sigmoid2(rv)), m, q);
-  const float2 u = mul2(mul2(q, inv_sqrt2(q)), mul2(sigmoid2(iv), xv));
+  const float2 u = mul2(sqrt2(q), mul2(sigmoid2(iv), xv));
   const float2 hn = fma2(add2(m, bc2(1.f)), h0, u);
   hb[0] = hn.x;
   if (ok1) hb[1] = hn.y;

@@ -27,23 +27,24 @@ def _pointers(tensors):
     return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
-def _sizes(tensors):
-    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
-
-
-def _check_list(what, name, tensors, like, dtypes, sizes=None):
-    assert len(tensors) == len(like), f"{what}: {len(like)} tensors, but {len(tensors)} of {name}"
+def _check_list(what, name, tensors, sizes, dev, dtypes):
+    """Contiguous tensors of the given element counts and types on one device."""
+    assert len(tensors) == len(sizes), f"{what}: {len(sizes)} tensors, but {len(tensors)} of {name}"
     for k, t in enumerate(tensors):
+        if t.dtype in dtypes and t.numel() == sizes[k] and t.get_device() == dev and \
+                t.is_contiguous():
+            continue
         if t.dtype not in dtypes:
             raise TypeError(f"{what}: {name}[{k}] is {t.dtype}, "
                             f"not one of {', '.join(map(str, dtypes))}")
         assert t.is_contiguous(), f"{what}: {name}[{k}] must be contiguous"
-        n = like[k].numel() if sizes is None else sizes[k]
-        assert t.numel() == n, f"{what}: {name}[{k}] has {t.numel()} elements, not {n}"
-        assert t.device == like[0].device, f"{what}: tensors on different devices"
+        assert t.numel() == sizes[k], \
+            f"{what}: {name}[{k}] has {t.numel()} elements, not {sizes[k]}"
+        raise AssertionError(f"{what}: tensors on different devices")
 
 
-_FLOATS = (torch.float32, torch.bfloat16)
+_CODES = {torch.float32: _lib.MQC_DTYPE_F32, torch.bfloat16: _lib.MQC_DTYPE_BF16}
+_FLOATS = tuple(_CODES)
 
 
 @torch.no_grad()
@@ -54,20 +55,23 @@ def grad_norm(grads: list[torch.Tensor], max_norm: float | None = None) -> torch
     grads = list(grads)
     if not grads:
         return torch.tensor([0.0, 1.0])
-    _lib.require_cuda(*grads, what="grad_norm")
-    _check_list("grad_norm", "grads", grads, grads, _FLOATS)
+    _lib.require_cuda(grads[0], what="grad_norm")
+    sizes = [g.numel() for g in grads]
+    _check_list("grad_norm", "grads", grads, sizes, grads[0].get_device(), _FLOATS)
     assert max_norm is None or max_norm >= 0, "max_norm must not be negative"
-    dev = grads[0].device
-    out = torch.empty(2, dtype=torch.float32, device=dev)
-    codes = (ctypes.c_int32 * len(grads))(*[_lib.dtype_code(g) for g in grads])
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    with torch.cuda.device(idx):  # the workspace depends on the device's SMs
-        nbytes = _lib.load().mqc_grad_norm_workspace_size(len(grads))
-        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)
-        _lib.call_on(dev, "mqc_grad_norm", len(grads), _sizes(grads), _pointers(grads), codes,
-                     -1.0 if max_norm is None else float(max_norm), out.data_ptr(),
-                     ws.data_ptr(), nbytes)
-    return out
+    return _grad_norm(grads, sizes, max_norm)
+
+
+def _grad_norm(grads, sizes, max_norm):
+    dev, n = grads[0].device, len(grads)
+    # 4-byte words: the partial sums (8-byte aligned), then the two results
+    nbytes = _lib.load().mqc_grad_norm_workspace_size(n)
+    out = torch.empty(nbytes // 4 + 2, dtype=torch.float32, device=dev)
+    _lib.call_on(dev.index, "mqc_grad_norm", n, (ctypes.c_int64 * n)(*sizes), _pointers(grads),
+                 (ctypes.c_int32 * n)(*[_CODES[g.dtype] for g in grads]),
+                 -1.0 if max_norm is None else float(max_norm), out.data_ptr() + nbytes,
+                 out.data_ptr(), nbytes)
+    return out[nbytes // 4:]
 
 
 @torch.no_grad()
@@ -102,48 +106,50 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     _lib.require_cuda(params[0], what=what)
     bits = 32 if exponents is None else 8
     state = (torch.float32,) if bits == 32 else (torch.uint8,)
-    _check_list(what, "params", params, params, _FLOATS)
-    _check_list(what, "grads", grads, params, _FLOATS)
-    _check_list(what, "exp_avgs", exp_avgs, params, state)
-    _check_list(what, "exp_avg_sqs", exp_avg_sqs, params, state)
+    sizes = [p.numel() for p in params]
+    idx = params[0].get_device()
+    _check_list(what, "params", params, sizes, idx, _FLOATS)
+    _check_list(what, "grads", grads, sizes, idx, _FLOATS)
+    _check_list(what, "exp_avgs", exp_avgs, sizes, idx, state)
+    _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, idx, state)
     lists = [params, grads, exp_avgs, exp_avg_sqs]
     if bits == 8:
-        blocks = [-(-p.numel() // _lib.MQC_ADAMW_BLOCK) for p in params]
+        blocks = [-(-n // _lib.MQC_ADAMW_BLOCK) for n in sizes]
         for name, part in zip(("exponents[0]", "exponents[1]"), exponents):
-            _check_list(what, name, part, params, (torch.uint8,), blocks)
+            _check_list(what, name, part, blocks, idx, state)
         lists += [list(exponents[0]), list(exponents[1])]
     if ordinals is None:
         ordinals = range(len(params))
     assert len(ordinals) == len(params), f"{what}: one ordinal a tensor"
-    dev = params[0].device
     norm = None
-    if max_grad_norm is not None:
-        got = grad_norm(grads, max_grad_norm)
-        norm, clip = got[0], got[1]
-    elif clip is not None:
-        assert clip.numel() == 1 and clip.dtype == torch.float32 and clip.device == dev, \
-            "clip must be one float32 on the parameters' device"
     a = _lib.AdamwArgs()
-    a.clip = _lib.ptr(clip)
+    if max_grad_norm is not None:
+        assert max_grad_norm >= 0, "max_norm must not be negative"
+        got = _grad_norm(grads, sizes, max_grad_norm)
+        norm, a.clip = got[0], got.data_ptr() + 4
+    elif clip is not None:
+        assert clip.numel() == 1 and clip.dtype == torch.float32 and clip.get_device() == idx, \
+            "clip must be one float32 on the parameters' device"
+        a.clip = clip.data_ptr()
     a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = lr, betas, eps, weight_decay
     a.step, a.state_bits, a.seed = step, bits, seed & 0xFFFFFFFF
     a.flags = _lib.MQC_ADAMW_CARRY if carry else 0
     # one call for each pair of parameter and gradient types
     kinds: dict[tuple[int, int], list[int]] = {}
     for k, (p, g) in enumerate(zip(params, grads)):
-        kinds.setdefault((_lib.dtype_code(p), _lib.dtype_code(g)), []).append(k)
-    for (a.param_dtype, a.grad_dtype), members in kinds.items():
-        whole = len(members) == len(params)
-        part = lists if whole else [[t[k] for k in members] for t in lists]
-        sizes = _sizes(part[0])
-        places = (ctypes.c_int64 * len(members))(*[ordinals[k] for k in members])
+        kinds.setdefault((p.dtype, g.dtype), []).append(k)
+    for (p_dtype, g_dtype), members in kinds.items():
+        n = len(members)
+        part = lists if n == len(params) else [[t[k] for k in members] for t in lists]
+        numel = (ctypes.c_int64 * n)(*[sizes[k] for k in members])
+        places = (ctypes.c_int64 * n)(*[ordinals[k] for k in members])
         arrays = [_pointers(t) for t in part]
-        a.count = len(members)
-        a.numel, a.ordinal = ctypes.addressof(sizes), ctypes.addressof(places)
+        a.count, a.param_dtype, a.grad_dtype = n, _CODES[p_dtype], _CODES[g_dtype]
+        a.numel, a.ordinal = ctypes.addressof(numel), ctypes.addressof(places)
         for field, arr in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent",
                                "exp_avg_sq_exponent"), arrays):
             setattr(a, field, ctypes.addressof(arr))
-        _lib.call_on(dev, "mqc_adamw_step", ctypes.byref(a))
+        _lib.call_on(idx, "mqc_adamw_step", ctypes.byref(a))
     return norm
 
 
@@ -157,15 +163,16 @@ def adamw_moments(exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
         return [], []
     what = "adamw_moments"
     _lib.require_cuda(exp_avgs[0], what=what)
-    _check_list(what, "exp_avgs", exp_avgs, exp_avgs, (torch.uint8,))
-    _check_list(what, "exp_avg_sqs", exp_avg_sqs, exp_avgs, (torch.uint8,))
-    blocks = [-(-t.numel() // _lib.MQC_ADAMW_BLOCK) for t in exp_avgs]
+    sizes = [t.numel() for t in exp_avgs]
+    idx, n = exp_avgs[0].get_device(), len(exp_avgs)
+    _check_list(what, "exp_avgs", exp_avgs, sizes, idx, (torch.uint8,))
+    _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, idx, (torch.uint8,))
+    blocks = [-(-k // _lib.MQC_ADAMW_BLOCK) for k in sizes]
     for name, part in zip(("exponents[0]", "exponents[1]"), exponents):
-        _check_list(what, name, part, exp_avgs, (torch.uint8,), blocks)
-    dev = exp_avgs[0].device
-    m, root = ([torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in exp_avgs]
-               for _ in range(2))
-    _lib.call_on(dev, "mqc_adamw_moments", len(exp_avgs), _sizes(exp_avgs), _pointers(exp_avgs),
+        _check_list(what, name, part, blocks, idx, (torch.uint8,))
+    m = [torch.empty_like(t, dtype=torch.bfloat16) for t in exp_avgs]
+    root = [torch.empty_like(t, dtype=torch.bfloat16) for t in exp_avgs]
+    _lib.call_on(idx, "mqc_adamw_moments", n, (ctypes.c_int64 * n)(*sizes), _pointers(exp_avgs),
                  _pointers(exp_avg_sqs), _pointers(exponents[0]), _pointers(exponents[1]),
                  _pointers(m), _pointers(root))
     return m, root

@@ -17,40 +17,56 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .block_fused import _rows
 
 __all__ = ["gated_linear_scan", "gated_linear_step"]
 
+_F32 = torch.float32
+_CODES = {torch.float32: _lib.MQC_DTYPE_F32, torch.bfloat16: _lib.MQC_DTYPE_BF16}
+
 
 def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
     """Contiguous fp32 (the tensor itself where it is that already)."""
-    return None if t is None else t.detach().to(torch.float32).contiguous()
+    if t is None or (t.dtype is _F32 and t.is_contiguous()):
+        return t
+    return t.detach().to(_F32).contiguous()
+
+
+def _placed(t: torch.Tensor, dm: int):
+    """(tensor, row stride) of a tensor whose rows the kernel can read in place."""
+    if t.is_contiguous():
+        return t, dm
+    t, row = _rows(t)
+    return t, max(row, dm)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _forward(x, r, i, lam, h0, reset, sharpness, want_state, keep):
     """(y, hT, saved): ``keep`` leaves the states that the backward pass starts from."""
     bsz, seqlen, dm = x.shape
-    xs, x_row = _rows(x)
-    rs, r_row = _rows(r)
-    si, i_row = _rows(i)
+    xs, x_row = _placed(x, dm)
+    rs, r_row = _placed(r, dm)
+    si, i_row = _placed(i, dm)
     dev = x.device
-    y = torch.empty(bsz, seqlen, dm, dtype=x.dtype, device=dev)
-    hT = torch.empty(bsz, dm, dtype=torch.float32, device=dev) if want_state else None
-    ckpt = None
+    y = _like(x)
+    hT = ckpt = None
+    if want_state:
+        hT = torch.empty((bsz, dm), dtype=_F32, device=dev)
     if keep:
         tiles = -(-seqlen // _lib.MQC_GATED_SCAN_TILE)
-        ckpt = torch.empty(bsz, tiles, dm, dtype=torch.float32, device=dev)
-    a = _lib.GatedScanArgs()
-    a.batch, a.seq_len, a.channels = bsz, seqlen, dm
-    a.dtype, a.sharpness = _lib.dtype_code(x), sharpness
-    a.x, a.r, a.i = xs.data_ptr(), rs.data_ptr(), si.data_ptr()
-    a.x_row, a.r_row, a.i_row = max(x_row, dm), max(r_row, dm), max(i_row, dm)
-    a.lambda_, a.h0, a.reset = lam.data_ptr(), _lib.ptr(h0), _lib.ptr(reset)
-    a.y, a.hT, a.ckpt = y.data_ptr(), _lib.ptr(hT), _lib.ptr(ckpt)
+        ckpt = torch.empty((bsz, tiles, dm), dtype=_F32, device=dev)
+    ptr = _lib.ptr
+    a = _lib.GatedScanArgs(bsz, seqlen, dm, _CODES[x.dtype], sharpness, xs.data_ptr(),
+                           rs.data_ptr(), si.data_ptr(), x_row, r_row, i_row, lam.data_ptr(),
+                           ptr(h0), ptr(reset), y.data_ptr(), ptr(hT), ptr(ckpt))
     a.status = _lib.status_word(dev).data_ptr()
-    _lib.call_on(dev, "mqc_gated_scan_fwd", ctypes.byref(a))
+    _lib.call_on(dev.index, "mqc_gated_scan_fwd", ctypes.byref(a))
     return y, hT, (xs, rs, si, ckpt)
 
 
@@ -61,51 +77,56 @@ class _GatedScan(torch.autograd.Function):
         y, hT, (xs, rs, si, ckpt) = _forward(x, r, i, lam, _f32(h0), reset, sharpness, want_state,
                                              True)
         ctx.save_for_backward(xs, rs, si, lam, reset, ckpt)
-        ctx.sharpness = sharpness
-        ctx.meta = (Lambda.dtype, None if h0 is None else h0.dtype)
+        ctx.meta = (sharpness, Lambda.dtype, None if h0 is None else h0.dtype)
         ctx.set_materialize_grads(False)
         return y, hT
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dhT):
         xs, rs, si, lam, reset, ckpt = ctx.saved_tensors
         bsz, seqlen, dm = xs.shape
-        lam_dtype, h0_dtype = ctx.meta
+        sharpness, lam_dtype, h0_dtype = ctx.meta
         dev = xs.device
-        x_row, r_row, i_row = (_rows(t)[1] for t in (xs, rs, si))
-        dys, dy_row = (None, 0) if dy is None else _rows(dy.to(xs.dtype))
+        dy_row = dm
+        if dy is not None:
+            dy, dy_row = _placed(dy if dy.dtype is xs.dtype else dy.to(xs.dtype), dm)
         dhT = _f32(dhT)
-        dx, dr, di = (torch.empty(bsz, seqlen, dm, dtype=xs.dtype, device=dev) for _ in range(3))
-        dlam = torch.empty(dm, dtype=torch.float32, device=dev)
+        dx, dr, di = _like(xs), _like(xs), _like(xs)
+        nbytes = _lib.load().mqc_gated_scan_bwd_workspace_size(bsz, seqlen, dm)
+        ws = torch.empty(max(1, nbytes // 4), dtype=_F32, device=dev)
+        dlam = torch.empty_like(lam)
         dh0 = None
         if h0_dtype is not None and ctx.needs_input_grad[4]:
-            dh0 = torch.empty(bsz, dm, dtype=torch.float32, device=dev)
-        nbytes = _lib.load().mqc_gated_scan_bwd_workspace_size(bsz, seqlen, dm)
-        ws = torch.empty(max(1, nbytes // 4), dtype=torch.float32, device=dev)
-        a = _lib.GatedScanArgs()
-        a.batch, a.seq_len, a.channels = bsz, seqlen, dm
-        a.dtype, a.sharpness = _lib.dtype_code(xs), ctx.sharpness
-        a.x, a.r, a.i = xs.data_ptr(), rs.data_ptr(), si.data_ptr()
-        a.x_row, a.r_row, a.i_row = max(x_row, dm), max(r_row, dm), max(i_row, dm)
-        a.lambda_, a.reset, a.ckpt = lam.data_ptr(), _lib.ptr(reset), ckpt.data_ptr()
-        a.dy, a.dy_row, a.dhT = _lib.ptr(dys), max(dy_row, dm), _lib.ptr(dhT)
-        a.dx, a.dr, a.di = dx.data_ptr(), dr.data_ptr(), di.data_ptr()
-        a.dlambda, a.dh0 = dlam.data_ptr(), _lib.ptr(dh0)
-        a.status = _lib.status_word(dev).data_ptr()
-        _lib.call_on(dev, "mqc_gated_scan_bwd", ctypes.byref(a), ws.data_ptr(), nbytes)
-        return (dx, dr, di, dlam.to(lam_dtype), None if dh0 is None else dh0.to(h0_dtype),
-                None, None, None)
+            dh0 = torch.empty((bsz, dm), dtype=_F32, device=dev)
+        ptr = _lib.ptr
+        a = _lib.GatedScanArgs(bsz, seqlen, dm, _CODES[xs.dtype], sharpness, xs.data_ptr(),
+                               rs.data_ptr(), si.data_ptr(), _placed(xs, dm)[1],
+                               _placed(rs, dm)[1], _placed(si, dm)[1], lam.data_ptr(), None,
+                               ptr(reset), None, None, ckpt.data_ptr(), ptr(dy), ptr(dhT), dy_row,
+                               dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dlam.data_ptr(),
+                               ptr(dh0), _lib.status_word(dev).data_ptr())
+        _lib.call_on(dev.index, "mqc_gated_scan_bwd", ctypes.byref(a), ws.data_ptr(), nbytes)
+        if lam_dtype is not _F32:
+            dlam = dlam.to(lam_dtype)
+        if dh0 is not None and h0_dtype is not _F32:
+            dh0 = dh0.to(h0_dtype)
+        return dx, dr, di, dlam, dh0, None, None, None
 
 
 def _check(what, x, r, i, Lambda, h):
-    assert r.shape == x.shape and i.shape == x.shape, f"{what}: x, r and i must have one shape"
-    assert r.dtype == x.dtype and i.dtype == x.dtype, f"{what}: x, r and i must have one dtype"
-    assert tuple(Lambda.shape) == (x.shape[-1],), f"{what}: Lambda must be [D]"
-    assert h is None or tuple(h.shape) == (x.shape[0], x.shape[-1]), f"{what}: state must be [B, D]"
-    _lib.dtype_code(x)
-    _lib.require_cuda(x, r, i, Lambda, h, what=what)
-    for t in (r, i, Lambda, h):
-        assert t is None or t.device == x.device, f"{what}: tensors on different devices"
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    assert r.shape == shape and i.shape == shape, f"{what}: x, r and i must have one shape"
+    assert r.dtype is dtype and i.dtype is dtype, f"{what}: x, r and i must have one dtype"
+    assert Lambda.dim() == 1 and Lambda.numel() == shape[-1], f"{what}: Lambda must be [D]"
+    assert h is None or (h.dim() == 2 and h.shape[0] == shape[0] and h.shape[1] == shape[-1]), \
+        f"{what}: state must be [B, D]"
+    if dtype not in _CODES:
+        _lib.dtype_code(x)
+    if dev < 0:
+        _lib.require_cuda(x, what=what)
+    assert r.get_device() == dev and i.get_device() == dev and Lambda.get_device() == dev and \
+        (h is None or h.get_device() == dev), f"{what}: tensors on different devices"
 
 
 def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda: torch.Tensor,
@@ -128,8 +149,9 @@ def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda:
             "reset must be bool [B, T]"
         assert reset.device == x.device, "gated_linear_scan: tensors on different devices"
         reset = reset.contiguous()
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, r, i, Lambda, h0)):
+    if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or
+                                    Lambda.requires_grad or
+                                    (h0 is not None and h0.requires_grad)):
         y, hT = _GatedScan.apply(x, r, i, Lambda, h0, reset, float(sharpness),
                                  return_final_state)
     else:
@@ -138,27 +160,27 @@ def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda:
     return (y, hT) if return_final_state else y
 
 
-@torch.no_grad()
 def gated_linear_step(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda: torch.Tensor,
                       h: torch.Tensor, *, sharpness: float = 8.0,
                       out: torch.Tensor | None = None) -> torch.Tensor:
     """One token of B sequences: x, r, i [B, D]; the state h [B, D] fp32 is advanced
-    in place. Returns y [B, D] in x's dtype (``out`` if given). No gradient."""
+    in place. Returns y [B, D] in x's dtype (``out`` if given). Has no gradient: what
+    requires one is read as it stands."""
     assert x.dim() == 2, f"x must be [B, D], got {tuple(x.shape)}"
     _check("gated_linear_step", x, r, i, Lambda, h)
     assert sharpness > 0, "sharpness must be positive"
     assert h is not None and h.dtype == torch.float32 and h.is_contiguous(), \
         "h must be a contiguous float32 [B, D] state"
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _like(x.detach() if x.requires_grad else x)
     else:
         assert out.shape == x.shape and out.dtype == x.dtype and out.is_contiguous() and \
             out.device == x.device, "out must be a contiguous tensor like x"
     bsz, dm = x.shape
-    x, x_row = _rows(x)
-    r, r_row = _rows(r)
-    i, i_row = _rows(i)
-    _lib.call_on(x.device, "mqc_gated_scan_step", x.data_ptr(), max(x_row, dm), r.data_ptr(),
-                 max(r_row, dm), i.data_ptr(), max(i_row, dm), _f32(Lambda).data_ptr(),
-                 h.data_ptr(), out.data_ptr(), bsz, dm, float(sharpness), _lib.dtype_code(x))
+    x, x_row = _placed(x, dm)
+    r, r_row = _placed(r, dm)
+    i, i_row = _placed(i, dm)
+    _lib.call_on(x.get_device(), "mqc_gated_scan_step", x.data_ptr(), x_row, r.data_ptr(), r_row,
+                 i.data_ptr(), i_row, _f32(Lambda).data_ptr(), h.data_ptr(), out.data_ptr(), bsz,
+                 dm, float(sharpness), _CODES[x.dtype])
     return out
