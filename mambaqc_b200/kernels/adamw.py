@@ -23,24 +23,29 @@ from .. import _lib
 __all__ = ["adamw_step", "adamw_moments", "grad_norm"]
 
 
+_Tensor = torch.Tensor
+
+
 def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+    return (ctypes.c_void_p * len(tensors))(*map(_Tensor.data_ptr, tensors))
 
 
 def _check_list(what, name, tensors, sizes, dev, dtypes):
     """Contiguous tensors of the given element counts and types on one device."""
+    if (list(map(_Tensor.numel, tensors)) == sizes and
+            set(map(_Tensor.get_device, tensors)) == {dev} and
+            all(map(_Tensor.is_contiguous, tensors)) and
+            all([t.dtype in dtypes for t in tensors])):
+        return
     assert len(tensors) == len(sizes), f"{what}: {len(sizes)} tensors, but {len(tensors)} of {name}"
     for k, t in enumerate(tensors):
-        if t.dtype in dtypes and t.numel() == sizes[k] and t.get_device() == dev and \
-                t.is_contiguous():
-            continue
         if t.dtype not in dtypes:
             raise TypeError(f"{what}: {name}[{k}] is {t.dtype}, "
                             f"not one of {', '.join(map(str, dtypes))}")
         assert t.is_contiguous(), f"{what}: {name}[{k}] must be contiguous"
         assert t.numel() == sizes[k], \
             f"{what}: {name}[{k}] has {t.numel()} elements, not {sizes[k]}"
-        raise AssertionError(f"{what}: tensors on different devices")
+        assert t.get_device() == dev, f"{what}: tensors on different devices"
 
 
 _CODES = {torch.float32: _lib.MQC_DTYPE_F32, torch.bfloat16: _lib.MQC_DTYPE_BF16}
@@ -56,7 +61,7 @@ def grad_norm(grads: list[torch.Tensor], max_norm: float | None = None) -> torch
     if not grads:
         return torch.tensor([0.0, 1.0])
     _lib.require_cuda(grads[0], what="grad_norm")
-    sizes = [g.numel() for g in grads]
+    sizes = list(map(_Tensor.numel, grads))
     _check_list("grad_norm", "grads", grads, sizes, grads[0].get_device(), _FLOATS)
     assert max_norm is None or max_norm >= 0, "max_norm must not be negative"
     return _grad_norm(grads, sizes, max_norm)
@@ -106,7 +111,7 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     _lib.require_cuda(params[0], what=what)
     bits = 32 if exponents is None else 8
     state = (torch.float32,) if bits == 32 else (torch.uint8,)
-    sizes = [p.numel() for p in params]
+    sizes = list(map(_Tensor.numel, params))
     idx = params[0].get_device()
     _check_list(what, "params", params, sizes, idx, _FLOATS)
     _check_list(what, "grads", grads, sizes, idx, _FLOATS)
@@ -135,14 +140,21 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     a.step, a.state_bits, a.seed = step, bits, seed & 0xFFFFFFFF
     a.flags = _lib.MQC_ADAMW_CARRY if carry else 0
     # one call for each pair of parameter and gradient types
-    kinds: dict[tuple[int, int], list[int]] = {}
-    for k, (p, g) in enumerate(zip(params, grads)):
-        kinds.setdefault((p.dtype, g.dtype), []).append(k)
+    kinds: dict[tuple, list[int] | range] = {}
+    pairs = [(p.dtype, g.dtype) for p, g in zip(params, grads)]
+    if len(set(pairs)) == 1:
+        kinds[pairs[0]] = range(len(params))
+    else:
+        for k, pair in enumerate(pairs):
+            kinds.setdefault(pair, []).append(k)
     for (p_dtype, g_dtype), members in kinds.items():
         n = len(members)
-        part = lists if n == len(params) else [[t[k] for k in members] for t in lists]
-        numel = (ctypes.c_int64 * n)(*[sizes[k] for k in members])
-        places = (ctypes.c_int64 * n)(*[ordinals[k] for k in members])
+        part, count, place = lists, sizes, ordinals
+        if n < len(params):
+            part = [[t[k] for k in members] for t in lists]
+            count, place = [sizes[k] for k in members], [ordinals[k] for k in members]
+        numel = (ctypes.c_int64 * n)(*count)
+        places = (ctypes.c_int64 * n)(*place)
         arrays = [_pointers(t) for t in part]
         a.count, a.param_dtype, a.grad_dtype = n, _CODES[p_dtype], _CODES[g_dtype]
         a.numel, a.ordinal = ctypes.addressof(numel), ctypes.addressof(places)
@@ -163,7 +175,7 @@ def adamw_moments(exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
         return [], []
     what = "adamw_moments"
     _lib.require_cuda(exp_avgs[0], what=what)
-    sizes = [t.numel() for t in exp_avgs]
+    sizes = list(map(_Tensor.numel, exp_avgs))
     idx, n = exp_avgs[0].get_device(), len(exp_avgs)
     _check_list(what, "exp_avgs", exp_avgs, sizes, idx, (torch.uint8,))
     _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, idx, (torch.uint8,))
