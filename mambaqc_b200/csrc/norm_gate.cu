@@ -42,7 +42,7 @@ static_assert(kMaxWidth <= kMaxThreads * 8, "at most eight columns a thread");
 constexpr int kBwdThreads = 384;  // threads of a backward CTA (168 registers each) unless a row needs more
 constexpr bool kKeepBwd = true;
 constexpr int kFwdThreads = 256;  // threads of a forward CTA
-constexpr int kFwdCtas = 2;       // forward CTAs an SM, at most
+constexpr int kFwdCtas = 2;       // forward CTAs an SM, at most (they keep the parameters); without: 8
 constexpr int kFewRows = 8;       // rows an SM up to which a row is split over warps
 constexpr int kSums = 5;  // column sums: dwp, dscale, dbp, dwq, dbq
 
@@ -333,7 +333,7 @@ struct Ring {
 // read from L1 for each row they missed it often enough to cost as much L2 traffic as
 // the rows themselves.
 template <typename TX, typename TY, bool kVec, bool kPost, int K>
-__global__ void __launch_bounds__(kFwdThreads, kVec ? 2 : 1)
+__global__ void __launch_bounds__(kFwdThreads, kVec || K > 1 ? 2 : 4)
     norm_gate_fwd_kernel(const FwdArgs p) {
   __shared__ __align__(8) float red[2][kMaxWarps][2];
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -679,7 +679,7 @@ int launch_fwd_k(FwdArgs& f, cudaStream_t st) {
   auto kernel = norm_gate_fwd_kernel<TX, TY, kVec, kPost, K>;
   const size_t smem = K > 1 ? 5 * sizeof(float) * size_t(f.width) : 0;
   if (int rc = allow_smem(kernel, smem, "mqc_norm_gate_fwd")) return rc;
-  const int64_t most = int64_t(num_sms()) * kFwdCtas;
+  const int64_t most = int64_t(num_sms()) * (K > 1 ? kFwdCtas : 8);
   kernel<<<unsigned(ctas < most ? ctas : most), threads, smem, st>>>(f);
   return check_launch("mqc_norm_gate_fwd");
 }
