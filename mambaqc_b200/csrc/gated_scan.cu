@@ -303,7 +303,7 @@ constexpr int kFwdWarps = 8;
 
 template <typename T>
 struct FwdSmem {
-  T raw[2][3][kTile][kChan];          // x, r, i of this tile and the next
+  T raw[3][kTile][kChan];             // x, r, i of a tile
   float2 run[kFwdWarps][kChan];       // (M, E) of each warp's run
   float start[kFwdWarps][kChan];      // state before each run
   Exchange<kMaxCluster<T>> ex;
@@ -312,7 +312,7 @@ struct FwdSmem {
 // One tile: (A) each warp reduces its run to (M, E); (B) one thread a channel joins
 // the runs, exchanges the tile's pair with the cluster and hands each run its start;
 // (C) each warp runs its steps again from there and stores y. The next tile's copies
-// are in flight meanwhile.
+// are in flight from (B) on.
 template <typename T, int kBytes, bool kVec, bool kReset>
 __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     gated_scan_fwd_kernel(const FwdArgs p) {
@@ -341,16 +341,16 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
   const bool jok = tid < kChan && jc < p.channels;
   float carry = jok && p.h0 ? p.h0[int64_t(b) * p.channels + jc] : 0.f;
 
-  auto load = [&](int tile, int st) {
+  auto load = [&](int tile) {
     const int64_t t0 = int64_t(tile) * kTile;
     const int rows = p.seq - int(t0), cols = p.channels - c0;
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][0][0][0], x + t0 * p.xs, p.xs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][1][0][0], r + t0 * p.rs, p.rs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][2][0][0], iv + t0 * p.is, p.is, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[0][0][0], x + t0 * p.xs, p.xs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[1][0][0], r + t0 * p.rs, p.rs, rows, cols);
+    copy_tile<T, kBytes, kThreads>(&sm.raw[2][0][0], iv + t0 * p.is, p.is, rows, cols);
   };
 
   if (csize > 1) exchange_init(&sm.ex);
-  if (rank < tiles) load(rank, 0);
+  if (rank < tiles) load(rank);
   cp_async_commit();
   if (csize > 1) cluster.sync();  // every CTA's mbarriers are ready before they are written
   bool alive = true;
@@ -359,9 +359,7 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     const int tile = first + rank, st = round & 1;
     const int t0 = tile * kTile + warp * S;
     cp_async_wait_all();
-    __syncthreads();  // the tile has landed; the other buffer is no longer read
-    if (tile + csize < tiles) load(tile + csize, st ^ 1);
-    cp_async_commit();
+    __syncthreads();  // the tile has landed
     float2 a[S], u[S];
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f);
@@ -372,9 +370,9 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
         const int row = warp * S + s;
         const bool in = decltype(whole)::value || t0 + s < p.seq;
         float2 m, q;
-        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]))), m, q);
+        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[1][row][2 * lane]))), m, q);
         const float2 v =
-            mul2(sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane])), unpack2(&sm.raw[st][0][row][2 * lane]));
+            mul2(sigmoid2(unpack2(&sm.raw[2][row][2 * lane])), unpack2(&sm.raw[0][row][2 * lane]));
         u[s] = mul2(sqrt2(q), v);
         drop[s] = kReset && in && rst[t0 + s] != 0;
         if (!in) m = u[s] = bc2(0.f);
@@ -392,7 +390,9 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     if (whole) reduce(std::true_type{});
     else if (tile < tiles) reduce(std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
-    __syncthreads();
+    __syncthreads();  // the runs are there, and the tile's rows are no longer read
+    if (tile + csize < tiles) load(tile + csize);
+    cp_async_commit();
     if (tid < kChan) {
       float h = carry;
       if (csize > 1) {
@@ -688,11 +688,13 @@ __global__ void __launch_bounds__(128)
 
 // ----------------------------------------------------------------------- host
 
-// How many clusters of 1, 2, 4, 8, 16 CTAs of a kernel fit the device at once
-// (asked once for each kernel and device; a repeated question gives the same answer).
+// How many clusters of each size of a kernel fit the device at once (asked once for
+// each kernel and device; a repeated question gives the same answer).
+constexpr int kSizes[] = {1, 2, 3, 4, 5, 6, 7, 8, 12, 16};
+constexpr int kSizeCount = int(sizeof(kSizes) / sizeof(int));
 struct Fit {
   std::atomic<int> known{0};
-  std::atomic<int> clusters[5];
+  std::atomic<int> clusters[kSizeCount];
 };
 
 cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, int64_t grid, int threads, size_t smem,
@@ -714,11 +716,11 @@ template <typename K>
 void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (most > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  for (int k = 0; k < 5; ++k) {
+  for (int k = 0; k < kSizeCount; ++k) {
     int n = 0;
     cudaLaunchAttribute at;
-    const cudaLaunchConfig_t cfg = cluster_config(&at, 1 << k, threads, smem, 1 << k, nullptr);
-    if ((1 << k) > most || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    const cudaLaunchConfig_t cfg = cluster_config(&at, kSizes[k], threads, smem, kSizes[k], nullptr);
+    if (kSizes[k] > most || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
     cudaGetLastError();
     fit.clusters[k].store(n);
   }
@@ -727,7 +729,9 @@ void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
 
 // Launches `units` clusters, one for each 64 channels of a sequence. The CTAs of a
 // cluster take consecutive tiles; of the sizes that fit (no more CTAs than tiles) it
-// is the one that needs the fewest rounds of a tile. *size: the size taken.
+// is the one that takes the least time: waves of clusters x rounds of a tile x what a
+// round takes, which is its latency and the work of the CTAs that share an SM, about as
+// long each. *size: the size taken.
 template <auto kernel, typename A>
 int launch_clusters(const char* what, const A& args, int threads, size_t smem, int most,
                     int64_t units, int tiles, cudaStream_t st, int* size) {
@@ -739,13 +743,16 @@ int launch_clusters(const char* what, const A& args, int threads, size_t smem, i
   if (!fit.known.load()) ask_fit(kernel, threads, smem, most, fit);
   int c = 0;
   int64_t least = INT64_MAX;
-  for (int k = 0; k < 5 && (c == 0 || (1 << k) <= tiles); ++k) {
-    const int n = fit.clusters[k].load();
+  const int64_t sms = num_sms();
+  for (int k = 0; k < kSizeCount && (c == 0 || kSizes[k] <= tiles); ++k) {
+    const int64_t n = fit.clusters[k].load(), size = kSizes[k];
     if (n <= 0) continue;
-    const int64_t rounds = ((units + n - 1) / n) * ((tiles + (1 << k) - 1) >> k);
-    if (rounds < least) {
-      least = rounds;
-      c = 1 << k;
+    const int64_t waves = (units + n - 1) / n, resident = units < n ? units : n;
+    const int64_t shared = (resident * size + sms - 1) / sms;  // CTAs an SM
+    const int64_t time = waves * ((tiles + size - 1) / size) * (1 + shared);
+    if (time < least) {
+      least = time;
+      c = int(size);
     }
   }
   MQC_REQUIRE(c > 0, MQC_ERR_CUDA, "%s: the kernel does not fit the device", what);
