@@ -328,6 +328,12 @@ def aligned_contig(t: torch.Tensor, align: int = 16) -> torch.Tensor:
 _status_words: dict[int, torch.Tensor] = {}
 
 
+def status_ptr(idx: int) -> int:
+    """Address of device ``idx``'s status word."""
+    w = _status_words.get(idx)
+    return (status_word(torch.device("cuda", idx)) if w is None else w).data_ptr()
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 word the scan kernels OR MQC_DEVICE_STATUS_* bits into."""
     idx = device.index if device.index is not None else torch.cuda.current_device()

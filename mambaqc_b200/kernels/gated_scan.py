@@ -65,7 +65,7 @@ def _forward(x, r, i, lam, h0, reset, sharpness, want_state, keep):
     a = _lib.GatedScanArgs(bsz, seqlen, dm, _CODES[x.dtype], sharpness, xs.data_ptr(),
                            rs.data_ptr(), si.data_ptr(), x_row, r_row, i_row, lam.data_ptr(),
                            ptr(h0), ptr(reset), y.data_ptr(), ptr(hT), ptr(ckpt))
-    a.status = _lib.status_word(dev).data_ptr()
+    a.status = _lib.status_ptr(dev.index)
     _lib.call_on(dev.index, "mqc_gated_scan_fwd", ctypes.byref(a))
     return y, hT, (xs, rs, si, ckpt)
 
@@ -105,7 +105,7 @@ class _GatedScan(torch.autograd.Function):
                                _placed(rs, dm)[1], _placed(si, dm)[1], lam.data_ptr(), None,
                                ptr(reset), None, None, ckpt.data_ptr(), ptr(dy), ptr(dhT), dy_row,
                                dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dlam.data_ptr(),
-                               ptr(dh0), _lib.status_word(dev).data_ptr())
+                               ptr(dh0), _lib.status_ptr(dev.index))
         _lib.call_on(dev.index, "mqc_gated_scan_bwd", ctypes.byref(a), ws.data_ptr(), nbytes)
         if lam_dtype is not _F32:
             dlam = dlam.to(lam_dtype)

@@ -118,6 +118,22 @@ def _run(x, y, z, weight, bias, scale, next_weight, next_bias, norm, eps, out_dt
     return _forward(x, y, z, params, _KINDS[norm], eps, out_dtype, False)[:2]
 
 
+def _fits(x, tensors, vectors, norm, eps) -> bool:
+    """Whether ``_check`` would pass, without building its messages."""
+    shape, dev = x.shape, x.get_device()
+    if dev < 0 or norm not in _KINDS or not eps >= 0 or not shape or \
+            x.dtype not in _CODES or shape[-1] > _lib.MQC_NORM_GATE_MAX_WIDTH:
+        return False
+    width = shape[-1]
+    for t in tensors:
+        if t.shape != shape or t.dtype not in _CODES or t.get_device() != dev:
+            return False
+    for t in vectors:
+        if t is not None and (t.dim() != 1 or t.numel() != width or t.get_device() != dev):
+            return False
+    return True
+
+
 def _check(what, x, tensors, vectors, norm, eps):
     assert norm in _KINDS, f"{what}: norm must be 'layer' or 'rms', got {norm!r}"
     assert eps >= 0, f"{what}: eps must not be negative"
@@ -151,9 +167,10 @@ def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor, weight
     next_weight, next_bias [D]. x may be fp32 with bf16 y and z; an fp32 y takes a
     bf16 x to fp32. out is in x's dtype, n in y's. Computed in fp32 and rounded once:
     n is Q of out before it is rounded. Differentiable in every tensor."""
-    _check("norm_gate_residual", x, (("x", x), ("y", y), ("z", z)),
-           (("weight", weight), ("scale", scale), ("bias", bias), ("next_weight", next_weight),
-            ("next_bias", next_bias)), norm, eps)
+    if not _fits(x, (y, z), (weight, scale, bias, next_weight, next_bias), norm, eps):
+        _check("norm_gate_residual", x, (("x", x), ("y", y), ("z", z)),
+               (("weight", weight), ("scale", scale), ("bias", bias),
+                ("next_weight", next_weight), ("next_bias", next_bias)), norm, eps)
     assert next_bias is None or next_weight is not None, "next_bias needs next_weight"
     if x.dtype == torch.bfloat16 and y.dtype == torch.float32:
         x = x.float()
@@ -170,7 +187,8 @@ def residual_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     and bias [D]. Returned in ``dtype`` (x's if None; bf16 from an fp32 x for a block
     that computes in bf16). Differentiable."""
     assert weight is not None, "residual_norm needs a weight"
-    _check("residual_norm", x, (("x", x),), (("weight", weight), ("bias", bias)), norm, eps)
+    if not _fits(x, (), (weight, bias), norm, eps):
+        _check("residual_norm", x, (("x", x),), (("weight", weight), ("bias", bias)), norm, eps)
     dtype = x.dtype if dtype is None else dtype
     assert dtype in (torch.float32, torch.bfloat16), "dtype must be float32 or bfloat16"
     if x.dtype == torch.bfloat16 and dtype == torch.float32:
