@@ -278,20 +278,25 @@ def call(name: str, *args) -> None:
     check(getattr(lib, name)(*args), name)
 
 
-# the current stream's handle without building a torch.cuda.Stream (0.1 us against 2)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                      lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+_torch_ops = None
 
 
-def call_on(idx: int, name: str, *args) -> None:
-    """``call`` with device ``idx`` current and its current stream as the last argument."""
-    if idx == torch.cuda.current_device():
-        rc = getattr(_lib or load(), name)(*args, _raw_stream(idx))
-        if rc != MQC_OK:
-            check(rc, name)
-    else:
-        with torch.cuda.device(idx):
-            call(name, *args, _raw_stream(idx))
+def torch_ops():
+    """The torch extension (``csrc/torch/ops.cpp``), bound to this package's library."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        with _lock:
+            if _torch_ops is None:
+                try:
+                    from . import _torch_ops as ops
+                except ImportError as e:
+                    raise RuntimeError(
+                        "mambaqc_b200: the torch extension is not built; run "
+                        "`python -m mambaqc_b200.csrc.build`") from e
+                ops.init(str(LIB_PATH))
+                _torch_ops = ops
+    return _torch_ops
 
 
 def dtype_code(t: torch.Tensor) -> int:

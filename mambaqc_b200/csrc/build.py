@@ -8,7 +8,9 @@ Plain nvcc, in-tree, for sm_100a only:
 
 The library has a pure C ABI (``include/mambaqc_b200.h``) and links the CUDA
 runtime statically, so it carries no torch dependency; the Python package loads
-it with ctypes.
+it with ctypes. The operators of the training step are bound by a small torch
+extension beside it (``csrc/torch/ops.cpp`` -> ``mambaqc_b200/_torch_ops.so``, built
+with g++ against the installed torch), which calls the same C ABI.
 """
 
 from __future__ import annotations
@@ -27,6 +29,8 @@ ROOT = PKG.parent
 INCLUDE = ROOT / "include"
 BUILD_DIR = PKG / "_build"
 LIB = PKG / "libmambaqc_b200.so"
+OPS_SOURCE = CSRC / "torch" / "ops.cpp"
+OPS_LIB = PKG / "_torch_ops.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
@@ -89,7 +93,36 @@ def build(force: bool = False, jobs: int | None = None, quiet: bool = False) -> 
         os.replace(tmp, LIB)
         if not quiet:
             print(f"built {LIB}", file=sys.stderr)
+    build_torch_ops(force=force, quiet=quiet)
     return LIB
+
+
+def build_torch_ops(force: bool = False, quiet: bool = False) -> Path:
+    """The torch extension; compiled again when its source or the header is newer."""
+    newest = max(p.stat().st_mtime for p in (OPS_SOURCE, INCLUDE / "mambaqc_b200.h"))
+    if not force and OPS_LIB.exists() and OPS_LIB.stat().st_mtime >= newest:
+        return OPS_LIB
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda_home = Path(_nvcc()).resolve().parents[1]
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               cuda_home / "include", Path(sysconfig.get_paths()["include"]), INCLUDE]
+    tmp = OPS_LIB.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_torch_ops", *[f"-I{p}" for p in include], str(OPS_SOURCE),
+           "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch", "-ltorch_python", "-ldl"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for {OPS_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, OPS_LIB)
+    if not quiet:
+        print(f"built {OPS_LIB}", file=sys.stderr)
+    return OPS_LIB
 
 
 def main() -> None:

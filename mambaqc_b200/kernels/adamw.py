@@ -14,8 +14,6 @@ hash of (seed, step, tensor, element) that makes the rounding unbiased: v moves 
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from .. import _lib
@@ -23,20 +21,11 @@ from .. import _lib
 __all__ = ["adamw_step", "adamw_moments", "grad_norm"]
 
 
-_Tensor = torch.Tensor
-
-
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*map(_Tensor.data_ptr, tensors))
+_FLOATS = (torch.float32, torch.bfloat16)
 
 
 def _check_list(what, name, tensors, sizes, dev, dtypes):
     """Contiguous tensors of the given element counts and types on one device."""
-    if (list(map(_Tensor.numel, tensors)) == sizes and
-            set(map(_Tensor.get_device, tensors)) == {dev} and
-            all(map(_Tensor.is_contiguous, tensors)) and
-            all([t.dtype in dtypes for t in tensors])):
-        return
     assert len(tensors) == len(sizes), f"{what}: {len(sizes)} tensors, but {len(tensors)} of {name}"
     for k, t in enumerate(tensors):
         if t.dtype not in dtypes:
@@ -48,8 +37,8 @@ def _check_list(what, name, tensors, sizes, dev, dtypes):
         assert t.get_device() == dev, f"{what}: tensors on different devices"
 
 
-_CODES = {torch.float32: _lib.MQC_DTYPE_F32, torch.bfloat16: _lib.MQC_DTYPE_BF16}
-_FLOATS = tuple(_CODES)
+def _blocks(sizes):
+    return [-(-n // _lib.MQC_ADAMW_BLOCK) for n in sizes]
 
 
 @torch.no_grad()
@@ -61,22 +50,10 @@ def grad_norm(grads: list[torch.Tensor], max_norm: float | None = None) -> torch
     if not grads:
         return torch.tensor([0.0, 1.0])
     _lib.require_cuda(grads[0], what="grad_norm")
-    sizes = list(map(_Tensor.numel, grads))
-    _check_list("grad_norm", "grads", grads, sizes, grads[0].get_device(), _FLOATS)
+    _check_list("grad_norm", "grads", grads, [g.numel() for g in grads], grads[0].get_device(),
+                _FLOATS)
     assert max_norm is None or max_norm >= 0, "max_norm must not be negative"
-    return _grad_norm(grads, sizes, max_norm)
-
-
-def _grad_norm(grads, sizes, max_norm):
-    dev, n = grads[0].device, len(grads)
-    # 4-byte words: the partial sums (8-byte aligned), then the two results
-    nbytes = _lib.load().mqc_grad_norm_workspace_size(n)
-    out = torch.empty(nbytes // 4 + 2, dtype=torch.float32, device=dev)
-    _lib.call_on(dev.index, "mqc_grad_norm", n, (ctypes.c_int64 * n)(*sizes), _pointers(grads),
-                 (ctypes.c_int32 * n)(*[_CODES[g.dtype] for g in grads]),
-                 -1.0 if max_norm is None else float(max_norm), out.data_ptr() + nbytes,
-                 out.data_ptr(), nbytes)
-    return out[nbytes // 4:]
+    return _lib.torch_ops().grad_norm(grads, -1.0 if max_norm is None else float(max_norm))
 
 
 @torch.no_grad()
@@ -107,62 +84,42 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     assert max_grad_norm is None or clip is None, "max_grad_norm and clip exclude each other"
     if not params:
         return None if max_grad_norm is None else torch.zeros(())
-    what = "adamw_step"
-    _lib.require_cuda(params[0], what=what)
-    bits = 32 if exponents is None else 8
-    state = (torch.float32,) if bits == 32 else (torch.uint8,)
-    sizes = list(map(_Tensor.numel, params))
-    idx = params[0].get_device()
-    _check_list(what, "params", params, sizes, idx, _FLOATS)
-    _check_list(what, "grads", grads, sizes, idx, _FLOATS)
-    _check_list(what, "exp_avgs", exp_avgs, sizes, idx, state)
-    _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, idx, state)
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    if bits == 8:
-        blocks = [-(-n // _lib.MQC_ADAMW_BLOCK) for n in sizes]
-        for name, part in zip(("exponents[0]", "exponents[1]"), exponents):
-            _check_list(what, name, part, blocks, idx, state)
-        lists += [list(exponents[0]), list(exponents[1])]
+    ops = _lib.torch_ops()
+    bits8 = exponents is not None
+    em, ev = (list(exponents[0]), list(exponents[1])) if bits8 else ([], [])
+    if not ops.lists_fit(params, grads, exp_avgs, exp_avg_sqs, em, ev, bits8):
+        _refuse_lists(params, grads, exp_avgs, exp_avg_sqs, em, ev, bits8)
     if ordinals is None:
         ordinals = range(len(params))
-    assert len(ordinals) == len(params), f"{what}: one ordinal a tensor"
+    assert len(ordinals) == len(params), "adamw_step: one ordinal a tensor"
     norm = None
-    a = _lib.AdamwArgs()
     if max_grad_norm is not None:
         assert max_grad_norm >= 0, "max_norm must not be negative"
-        got = _grad_norm(grads, sizes, max_grad_norm)
-        norm, a.clip = got[0], got.data_ptr() + 4
+        got = ops.grad_norm(grads, float(max_grad_norm))
+        norm, clip = got[0], got[1]
     elif clip is not None:
-        assert clip.numel() == 1 and clip.dtype == torch.float32 and clip.get_device() == idx, \
+        assert clip.numel() == 1 and clip.dtype == torch.float32 and \
+            clip.get_device() == params[0].get_device(), \
             "clip must be one float32 on the parameters' device"
-        a.clip = clip.data_ptr()
-    a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = lr, betas, eps, weight_decay
-    a.step, a.state_bits, a.seed = step, bits, seed & 0xFFFFFFFF
-    a.flags = _lib.MQC_ADAMW_CARRY if carry else 0
-    # one call for each pair of parameter and gradient types
-    kinds: dict[tuple, list[int] | range] = {}
-    pairs = [(p.dtype, g.dtype) for p, g in zip(params, grads)]
-    if len(set(pairs)) == 1:
-        kinds[pairs[0]] = range(len(params))
-    else:
-        for k, pair in enumerate(pairs):
-            kinds.setdefault(pair, []).append(k)
-    for (p_dtype, g_dtype), members in kinds.items():
-        n = len(members)
-        part, count, place = lists, sizes, ordinals
-        if n < len(params):
-            part = [[t[k] for k in members] for t in lists]
-            count, place = [sizes[k] for k in members], [ordinals[k] for k in members]
-        numel = (ctypes.c_int64 * n)(*count)
-        places = (ctypes.c_int64 * n)(*place)
-        arrays = [_pointers(t) for t in part]
-        a.count, a.param_dtype, a.grad_dtype = n, _CODES[p_dtype], _CODES[g_dtype]
-        a.numel, a.ordinal = ctypes.addressof(numel), ctypes.addressof(places)
-        for field, arr in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_exponent",
-                               "exp_avg_sq_exponent"), arrays):
-            setattr(a, field, ctypes.addressof(arr))
-        _lib.call_on(idx, "mqc_adamw_step", ctypes.byref(a))
+    ops.adamw_step(params, grads, exp_avgs, exp_avg_sqs, em, ev, ordinals, clip, step, lr, betas[0],
+                   betas[1], eps, weight_decay, bits8, carry, seed & 0xFFFFFFFF)
     return norm
+
+
+def _refuse_lists(params, grads, exp_avgs, exp_avg_sqs, em, ev, bits8):
+    """Says what does not fit about the lists of a step."""
+    what = "adamw_step"
+    _lib.require_cuda(params[0], what=what)
+    state = (torch.uint8,) if bits8 else (torch.float32,)
+    sizes, dev = [p.numel() for p in params], params[0].get_device()
+    _check_list(what, "params", params, sizes, dev, _FLOATS)
+    _check_list(what, "grads", grads, sizes, dev, _FLOATS)
+    _check_list(what, "exp_avgs", exp_avgs, sizes, dev, state)
+    _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, dev, state)
+    if bits8:
+        _check_list(what, "exponents[0]", em, _blocks(sizes), dev, state)
+        _check_list(what, "exponents[1]", ev, _blocks(sizes), dev, state)
+    raise AssertionError(f"{what}: the lists do not fit together")
 
 
 @torch.no_grad()
@@ -175,16 +132,13 @@ def adamw_moments(exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
         return [], []
     what = "adamw_moments"
     _lib.require_cuda(exp_avgs[0], what=what)
-    sizes = list(map(_Tensor.numel, exp_avgs))
-    idx, n = exp_avgs[0].get_device(), len(exp_avgs)
-    _check_list(what, "exp_avgs", exp_avgs, sizes, idx, (torch.uint8,))
-    _check_list(what, "exp_avg_sqs", exp_avg_sqs, sizes, idx, (torch.uint8,))
-    blocks = [-(-k // _lib.MQC_ADAMW_BLOCK) for k in sizes]
-    for name, part in zip(("exponents[0]", "exponents[1]"), exponents):
-        _check_list(what, name, part, blocks, idx, (torch.uint8,))
-    m = [torch.empty_like(t, dtype=torch.bfloat16) for t in exp_avgs]
-    root = [torch.empty_like(t, dtype=torch.bfloat16) for t in exp_avgs]
-    _lib.call_on(idx, "mqc_adamw_moments", n, (ctypes.c_int64 * n)(*sizes), _pointers(exp_avgs),
-                 _pointers(exp_avg_sqs), _pointers(exponents[0]), _pointers(exponents[1]),
-                 _pointers(m), _pointers(root))
-    return m, root
+    em, ev = list(exponents[0]), list(exponents[1])
+    ops = _lib.torch_ops()
+    if not ops.lists_fit(exp_avgs, exp_avgs, exp_avgs, exp_avg_sqs, em, ev, True):
+        sizes, dev = [t.numel() for t in exp_avgs], exp_avgs[0].get_device()
+        for name, part, count in (("exp_avgs", exp_avgs, sizes),
+                                  ("exp_avg_sqs", exp_avg_sqs, sizes),
+                                  ("exponents[0]", em, _blocks(sizes)),
+                                  ("exponents[1]", ev, _blocks(sizes))):
+            _check_list(what, name, part, count, dev, (torch.uint8,))
+    return ops.adamw_moments(exp_avgs, exp_avg_sqs, em, ev)

@@ -12,121 +12,25 @@ stacks of blocks want both. The kernels are in ``csrc/norm_gate.cu``.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .block_fused import _rows
 
 __all__ = ["norm_gate_residual", "residual_norm"]
 
 _KINDS = {"layer": _lib.MQC_NORM_LAYER, "rms": _lib.MQC_NORM_RMS}
-
-
-_F32 = torch.float32
-_CODES = {torch.float32: _lib.MQC_DTYPE_F32, torch.bfloat16: _lib.MQC_DTYPE_BF16}
-
-
-def _param(t: torch.Tensor | None) -> torch.Tensor | None:
-    """Contiguous fp32 (the tensor itself where it is that already)."""
-    if t is None or (t.dtype is _F32 and t.is_contiguous()):
-        return t
-    return t.detach().to(_F32).contiguous()
-
-
-def _forward(x, y, z, params, kind, eps, out_dtype, keep):
-    """(out, n, x, y, z, z_row, stats); out is None without y, n without a next weight."""
-    width = x.shape[-1]
-    rows = x.numel() // width if width else 0
-    x = x.contiguous()
-    weight, bias, scale, next_weight, next_bias = params
-    out = n = stats = None
-    z_row = width
-    if y is not None:
-        y = y.contiguous()
-        if not z.is_contiguous():
-            z, z_row = _rows(z)
-            z_row = max(z_row, width)
-        out = torch.empty_like(x)
-    if next_weight is not None:
-        n = torch.empty_like(x, dtype=out_dtype)
-    if keep:
-        stats = torch.empty((rows, 4), dtype=_F32, device=x.device)
-    ptr = _lib.ptr
-    a = _lib.NormGateArgs(rows, width, z_row, _CODES[x.dtype], _CODES[out_dtype], kind, eps,
-                          x.data_ptr(), ptr(y), ptr(z), ptr(weight), ptr(bias), ptr(scale),
-                          ptr(next_weight), ptr(next_bias), ptr(out), ptr(n), ptr(stats))
-    _lib.call_on(x.get_device(), "mqc_norm_gate_fwd", ctypes.byref(a))
-    return out, n, x, y, z, z_row, stats
-
-
-class _NormGate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, z, weight, bias, scale, next_weight, next_bias, kind, eps, out_dtype):
-        raw = (weight, bias, scale, next_weight, next_bias)
-        params = tuple(map(_param, raw))
-        out, n, x, y, z, z_row, stats = _forward(x, y, z, params, kind, eps, out_dtype, True)
-        ctx.save_for_backward(x, y, z, stats, *params)
-        ctx.meta = (kind, eps, out_dtype, z_row,
-                    tuple(None if t is None else t.dtype for t in raw))
-        ctx.set_materialize_grads(False)
-        return out, n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dn):
-        x, y, z, stats, *params = ctx.saved_tensors
-        kind, eps, out_dtype, z_row, dtypes = ctx.meta
-        width = x.shape[-1]
-        rows = stats.shape[0]
-        dev = x.device
-        if dout is not None:
-            dout = (dout if dout.dtype is x.dtype else dout.to(x.dtype)).contiguous()
-        if dn is not None:
-            dn = (dn if dn.dtype is out_dtype else dn.to(out_dtype)).contiguous()
-        dx = torch.empty_like(x)
-        dy = dz = None
-        if y is not None:
-            dy, dz = torch.empty_like(y), torch.empty_like(y)
-        # needs_input_grad of weight, bias, scale, next_weight, next_bias
-        sums = [torch.empty_like(t) if t is not None and w else None
-                for t, w in zip(params, ctx.needs_input_grad[3:8])]
-        nbytes = _lib.load().mqc_norm_gate_bwd_workspace_size(rows, width)
-        ws = torch.empty(max(1, nbytes // 4), dtype=_F32, device=dev)
-        ptr = _lib.ptr
-        weight, bias, scale, next_weight, next_bias = map(ptr, params)
-        dweight, dbias, dscale, dnext_weight, dnext_bias = map(ptr, sums)
-        a = _lib.NormGateArgs(rows, width, z_row, _CODES[x.dtype], _CODES[out_dtype], kind, eps,
-                              x.data_ptr(), ptr(y), ptr(z), weight, bias, scale, next_weight,
-                              next_bias, None, None, stats.data_ptr(), ptr(dout), ptr(dn),
-                              dx.data_ptr(), ptr(dy), ptr(dz), dweight, dscale, dbias,
-                              dnext_weight, dnext_bias)
-        _lib.call_on(dev.index, "mqc_norm_gate_bwd", ctypes.byref(a), ws.data_ptr(), nbytes)
-        sums = [t if t is None or d is _F32 else t.to(d) for t, d in zip(sums, dtypes)]
-        return (dx, dy, dz, *sums, None, None, None)
-
-
-def _run(x, y, z, weight, bias, scale, next_weight, next_bias, norm, eps, out_dtype):
-    if torch.is_grad_enabled():
-        for t in (x, y, z, weight, bias, scale, next_weight, next_bias):
-            if t is not None and t.requires_grad:
-                return _NormGate.apply(x, y, z, weight, bias, scale, next_weight, next_bias,
-                                       _KINDS[norm], eps, out_dtype)
-    params = tuple(map(_param, (weight, bias, scale, next_weight, next_bias)))
-    return _forward(x, y, z, params, _KINDS[norm], eps, out_dtype, False)[:2]
+_TYPES = (torch.float32, torch.bfloat16)
 
 
 def _fits(x, tensors, vectors, norm, eps) -> bool:
     """Whether ``_check`` would pass, without building its messages."""
     shape, dev = x.shape, x.get_device()
     if dev < 0 or norm not in _KINDS or not eps >= 0 or not shape or \
-            x.dtype not in _CODES or shape[-1] > _lib.MQC_NORM_GATE_MAX_WIDTH:
+            x.dtype not in _TYPES or shape[-1] > _lib.MQC_NORM_GATE_MAX_WIDTH:
         return False
     width = shape[-1]
     for t in tensors:
-        if t.shape != shape or t.dtype not in _CODES or t.get_device() != dev:
+        if t.shape != shape or t.dtype not in _TYPES or t.get_device() != dev:
             return False
     for t in vectors:
         if t is not None and (t.dim() != 1 or t.numel() != width or t.get_device() != dev):
@@ -144,7 +48,7 @@ def _check(what, x, tensors, vectors, norm, eps):
         f"{what}: width {width} (at most {_lib.MQC_NORM_GATE_MAX_WIDTH})"
     for name, t in tensors:
         assert t.shape == shape, f"{what}: {name} must have x's shape"
-        if t.dtype not in _CODES:
+        if t.dtype not in _TYPES:
             _lib.dtype_code(t)
         assert t.get_device() == dev, f"{what}: tensors on different devices"
     for name, t in vectors:
@@ -166,7 +70,7 @@ def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor, weight
     (a column slice of a wider tensor is read in place); weight, scale, bias,
     next_weight, next_bias [D]. x may be fp32 with bf16 y and z; an fp32 y takes a
     bf16 x to fp32. out is in x's dtype, n in y's. Computed in fp32 and rounded once:
-    n is Q of out before it is rounded. Differentiable in every tensor."""
+    n is Q of out before it is rounded. Differentiable in every tensor (once)."""
     if not _fits(x, (y, z), (weight, scale, bias, next_weight, next_bias), norm, eps):
         _check("norm_gate_residual", x, (("x", x), ("y", y), ("z", z)),
                (("weight", weight), ("scale", scale), ("bias", bias),
@@ -176,7 +80,8 @@ def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor, weight
         x = x.float()
     if z.dtype != y.dtype:
         z = z.to(y.dtype)
-    out, n = _run(x, y, z, weight, bias, scale, next_weight, next_bias, norm, float(eps), y.dtype)
+    out, n = _lib.torch_ops().norm_gate(x, y, z, weight, bias, scale, next_weight, next_bias,
+                                        _KINDS[norm], float(eps), y.dtype is torch.float32)
     return out if next_weight is None else (out, n)
 
 
@@ -193,4 +98,5 @@ def residual_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     assert dtype in (torch.float32, torch.bfloat16), "dtype must be float32 or bfloat16"
     if x.dtype == torch.bfloat16 and dtype == torch.float32:
         x = x.float()
-    return _run(x, None, None, None, None, None, weight, bias, norm, float(eps), dtype)[1]
+    return _lib.torch_ops().norm_gate(x, None, None, None, None, None, weight, bias,
+                                      _KINDS[norm], float(eps), dtype is torch.float32)[1]

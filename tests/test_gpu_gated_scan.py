@@ -259,6 +259,20 @@ def test_gradient_against_differences():
         assert abs(got - want) < 2e-3 * abs(want), (k, got, want)
 
 
+def test_second_derivative_is_refused():
+    """The first derivative under create_graph is right; taking another from it raises."""
+    x, r, i, lam, h0, _ = map(_dev, _inputs(2, 70, 8, torch.float32))
+    leaves = [v.clone().requires_grad_() for v in (x, r, i, lam, h0)]
+    plain = torch.autograd.grad(gated_linear_scan(*leaves).sum(), leaves)
+    y = gated_linear_scan(*leaves)
+    g = torch.ones_like(y, requires_grad=True)
+    first = torch.autograd.grad(y, leaves, g, create_graph=True)
+    for a, b in zip(first, plain):
+        assert torch.equal(a.detach(), b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        first[0].sum().backward()
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("b,d", [(1, 1), (3, 33), (8, 64), (64, 1536)])
 def test_step_matches_scan(dt, b, d):

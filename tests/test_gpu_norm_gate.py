@@ -276,6 +276,18 @@ def test_gradient_against_differences():
             assert abs(got - want) < 2e-3 * abs(want), (kind, k, got, want)
 
 
+def test_second_derivative_is_refused():
+    q = {k: v.to(DEV).requires_grad_() for k, v in _inputs(4, 32, F32, F32, True, True).items()}
+    outs = _call(q, "layer")
+    grads = [torch.ones_like(o, requires_grad=True) for o in outs]
+    first = torch.autograd.grad(outs, list(q.values()), grads, create_graph=True)
+    plain = torch.autograd.grad(_call(q, "layer"), list(q.values()), [g.detach() for g in grads])
+    for a, b in zip(first, plain):
+        assert torch.equal(a.detach(), b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        first[1].sum().backward()
+
+
 def test_empty_rows():
     q = {k: v.to(DEV).requires_grad_() for k, v in _inputs(4, 32, F32, F32, True, True).items()}
     for k in "xyz":
