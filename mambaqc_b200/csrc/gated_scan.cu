@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <cmath>
 #include <initializer_list>
 #include <type_traits>
 
@@ -729,9 +730,11 @@ void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
 
 // Launches `units` clusters, one for each 64 channels of a sequence. The CTAs of a
 // cluster take consecutive tiles; of the sizes that fit (no more CTAs than tiles) it
-// is the one that takes the least time: waves of clusters x rounds of a tile x what a
-// round takes, which is its latency and the work of the CTAs that share an SM, about as
-// long each. *size: the size taken.
+// is the one that takes the least time by a model of waves of clusters x rounds of a
+// tile x what a round takes: 1.5 for its latency, 1 for each CTA that shares the SM,
+// and for the exchange 0.4 between two CTAs and 1.6 between more (in units of 0.8 us;
+// bf16 forward, us: 4 x 2048 x 1536 with 1, 2, 4 CTAs 62, 48, 35; 6 x 2048 x 1536 68, 50,
+// 58; 64 x 512 x 1024 72, 81, 101). *size: the size taken.
 template <auto kernel, typename A>
 int launch_clusters(const char* what, const A& args, int threads, size_t smem, int most,
                     int64_t units, int tiles, cudaStream_t st, int* size) {
@@ -742,15 +745,18 @@ int launch_clusters(const char* what, const A& args, int threads, size_t smem, i
   Fit& fit = fits[dev];
   if (!fit.known.load()) ask_fit(kernel, threads, smem, most, fit);
   int c = 0;
-  int64_t least = INT64_MAX;
-  const int64_t sms = num_sms();
+  double least = 0.0;
+  const double sms = num_sms();
   for (int k = 0; k < kSizeCount && (c == 0 || kSizes[k] <= tiles); ++k) {
     const int64_t n = fit.clusters[k].load(), size = kSizes[k];
     if (n <= 0) continue;
-    const int64_t waves = (units + n - 1) / n, resident = units < n ? units : n;
-    const int64_t shared = (resident * size + sms - 1) / sms;  // CTAs an SM
-    const int64_t time = waves * ((tiles + size - 1) / size) * (1 + shared);
-    if (time < least) {
+    const double exchange = size == 1 ? 0.0 : size == 2 ? 0.4 : 1.6;
+    auto wave = [&](int64_t u) {  // of u clusters
+      return u == 0 ? 0.0 : 1.5 + exchange + std::ceil(double(u * size) / sms);
+    };
+    const double time = double((tiles + size - 1) / size) *
+                        (double(units / n) * wave(n) + wave(units % n));
+    if (c == 0 || time < least) {
       least = time;
       c = int(size);
     }
