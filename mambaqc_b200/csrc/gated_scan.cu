@@ -732,12 +732,14 @@ void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
 // cluster take consecutive tiles; of the sizes that fit (no more CTAs than tiles) it
 // is the one that takes the least time by a model of waves of clusters x rounds of a
 // tile x what a round takes: 1.5 for its latency, 1 for each CTA that shares the SM,
-// and for the exchange 0.4 between two CTAs and 1.6 between more (in units of 0.8 us;
-// bf16 forward, us: 4 x 2048 x 1536 with 1, 2, 4 CTAs 62, 48, 35; 6 x 2048 x 1536 68, 50,
-// 58; 64 x 512 x 1024 72, 81, 101). *size: the size taken.
+// and `pair` for the exchange between two CTAs, `more` between more (forward 0.4 and 1.6
+// in units of 0.8 us; bf16, us: 4 x 2048 x 1536 with 1, 2, 4 CTAs 62, 48, 35; 6 x 2048 x
+// 1536 68, 50, 58; 64 x 512 x 1024 72, 81, 101; backward, whose rounds are longer, 0.5
+// and 0.75 in units of 1 us). *size: the size taken.
 template <auto kernel, typename A>
 int launch_clusters(const char* what, const A& args, int threads, size_t smem, int most,
-                    int64_t units, int tiles, cudaStream_t st, int* size) {
+                    int64_t units, int tiles, double pair, double more, cudaStream_t st,
+                    int* size) {
   static Fit fits[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -750,7 +752,7 @@ int launch_clusters(const char* what, const A& args, int threads, size_t smem, i
   for (int k = 0; k < kSizeCount && (c == 0 || kSizes[k] <= tiles); ++k) {
     const int64_t n = fit.clusters[k].load(), size = kSizes[k];
     if (n <= 0) continue;
-    const double exchange = size == 1 ? 0.0 : size == 2 ? 0.4 : 1.6;
+    const double exchange = size == 1 ? 0.0 : size == 2 ? pair : more;
     auto wave = [&](int64_t u) {  // of u clusters
       return u == 0 ? 0.0 : 1.5 + exchange + std::ceil(double(u * size) / sms);
     };
@@ -779,7 +781,7 @@ int run_fwd(const FwdArgs& f, cudaStream_t st) {
   int c;
   return launch_clusters<&gated_scan_fwd_kernel<T, kBytes, kVec, kReset>>(
       "mqc_gated_scan_fwd", f, kFwdWarps * 32, sizeof(FwdSmem<T>), kMaxCluster<T>,
-      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, st, &c);
+      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, 0.4, 1.6, st, &c);
 }
 
 template <typename T, int kBytes, bool kVec, bool kReset>
@@ -787,7 +789,7 @@ int run_bwd(const BwdArgs& f, float* dlambda, cudaStream_t st) {
   int c = 0;
   if (int rc = launch_clusters<&gated_scan_bwd_kernel<T, kBytes, kVec, kReset>>(
           "mqc_gated_scan_bwd", f, kBwdWarps * 32, sizeof(BwdSmem<T>), kMaxCluster<T>,
-          int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, st, &c))
+          int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, 0.5, 0.75, st, &c))
     return rc;
   gated_scan_dlambda_kernel<<<(f.channels + 31) / 32, 256, 0, st>>>(
       f.part, f.lambda, dlambda, f.batch * c, f.channels, f.sharpness);
