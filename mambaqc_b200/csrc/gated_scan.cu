@@ -11,16 +11,27 @@
 //
 // Layout. A CTA owns 64 channels of one sequence and walks over time in tiles of
 // kTile steps; each warp takes a run of consecutive steps of the tile, each lane
-// two channels, so every row access of a warp is one 128-byte (bf16) or 256-byte
-// (fp32) line and the arithmetic is packed two-wide. A run is reduced to (A, E),
-// h_out = A h_in + E (held as A - 1), in registers; runs are joined through shared memory, tiles
-// through the shared memory of a thread-block cluster whose CTAs take consecutive
-// tiles of the same sequence. So each input is read once and each output written
-// once, and no CTA waits for another one outside its cluster.
+// two channels, so the arithmetic is packed two-wide; the tile's rows come through
+// shared memory (cp.async). A run is reduced to (A, E), h_out = A h_in + E (held as
+// A - 1), in registers; runs are joined through shared memory, tiles through the
+// shared memory of a thread-block cluster whose CTAs take consecutive tiles of the same
+// sequence. So each input is read once and each output written once, and no CTA waits
+// for another one outside its cluster.
 //
 // The backward pass reads no y: it runs each tile again from the fp32 state that
 // the forward pass left at the tile's start (y in bf16 would cost dLambda three
 // digits), and the reverse recurrence uses the same products A.
+//
+// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 35 us, backward 79 us (and 3 for
+// dLambda), where the bytes alone take 15 and 27 us at 6.5 TB/s; 1 x 32768 x 1024
+// forward 133 us (41). Neither memory bounds it (with all tiles read from the cache and
+// nothing stored the forward takes 34 us) nor the special functions (35 us without any)
+// nor one pipe (the fullest, FMA, is 46 % busy), but the phases of a tile between
+// barriers: 47 instructions an element at 0.57 a cycle and scheduler with 24 warps an
+// SM. Slower or the same: four CTAs an SM at 64 registers (40 us), every warp joining
+// the runs for itself (38 us), an mbarrier for each rank (39 us; the long prefill 198),
+// unpacked arithmetic (40 us), one reciprocal for both sigmoids (37 us); backward with
+// eight warps of eight steps (82 us) or two CTAs an SM at 64 registers (109 us).
 #include <cooperative_groups.h>
 
 #include <atomic>

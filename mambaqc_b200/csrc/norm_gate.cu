@@ -20,6 +20,12 @@
 // row would need 120 registers for the sums alone); the rows of the next two steps are
 // on their way into shared memory meanwhile. Rows are dealt to CTAs by a fixed rule and
 // the CTAs' column sums are joined by a second kernel in a fixed order.
+//
+// Measured on one B200, LayerNorm, 8192 x 768, x fp32, y and z bf16: forward 18.7 us
+// (13.5 us of bytes at 6.5 TB/s), backward 38.1 and 3.5 us (21.2); RMSNorm, 16384 x 1024,
+// bf16: 30.3 (25.7), 60.3 and 3.7 us (41). The backward pass waits: 12 warps an SM (168
+// registers), two sums over a group with a barrier each for every row. Slower: 128
+// registers with spills (63 us), four columns a thread (44 us), 8 warps an SM (46 us).
 #include <type_traits>
 
 #include "mqc_common.cuh"
@@ -40,7 +46,6 @@ constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxWidth = MQC_NORM_GATE_MAX_WIDTH;
 static_assert(kMaxWidth <= kMaxThreads * 8, "at most eight columns a thread");
 constexpr int kBwdThreads = 384;  // threads of a backward CTA (168 registers each) unless a row needs more
-constexpr bool kKeepBwd = true;
 constexpr int kFwdThreads = 256;  // threads of a forward CTA
 constexpr int kFwdCtas = 2;       // forward CTAs an SM, at most (they keep the parameters); without: 8
 constexpr int kFewRows = 8;       // rows an SM up to which a row is split over warps
@@ -207,29 +212,6 @@ struct Place {
     } else {
 #pragma unroll
       for (int j = 0; j < kCols; ++j) mask |= uint32_t(first + j * step < width) << j;
-    }
-  }
-};
-
-// A parameter's values at this thread's columns: kept in registers (kKeep), or read
-// again from L1 for each row where the registers are needed for the rows themselves.
-template <bool kVec, bool kKeep>
-struct Cols {
-  const float* p;
-  Row<float, kVec> r;
-  __device__ __forceinline__ Cols(const float* ptr, const Place<kVec>& at)
-      : p(ptr != nullptr ? ptr + at.first : nullptr) {
-    r.zero();
-    if (kKeep && p != nullptr) r.load(p, at.step, at.mask);
-  }
-  __device__ __forceinline__ void get(float2 (&o)[4], const Place<kVec>& at) const {
-    if (kKeep) {
-      r.get(o);
-    } else {
-      Row<float, kVec> t;
-      t.zero();
-      if (p != nullptr) t.load(p, at.step, at.mask);
-      t.get(o);
     }
   }
 };
@@ -459,9 +441,11 @@ __global__ void __launch_bounds__(kBound)
   const Place<kVec> at(grp, p.width);
   const bool layer = p.layer != 0, next = p.dn != nullptr;
   const float inv = 1.f / float(p.width);
-  using C = Cols<kVec, kKeepBwd>;
-  const C wps(kPost ? p.wp : nullptr, at), bps(kPost ? p.bp : nullptr, at),
-      scs(kPost ? p.scale : nullptr, at), wqs(p.wq, at);
+  float2 wp[4], bp[4], sc[4], wq[4];
+  load_cols(kPost ? p.wp : nullptr, at, wp);
+  load_cols(kPost ? p.bp : nullptr, at, bp);
+  load_cols(kPost ? p.scale : nullptr, at, sc);
+  load_cols(p.wq, at, wq);
   float2 cs[kSums][4];
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
@@ -501,7 +485,7 @@ __global__ void __launch_bounds__(kBound)
     if (kVec) cp_async_wait_group<1>();
     const int64_t off = row * p.width + at.first;
     // d: dout, then the whole gradient of out; yh: yhat; gt: s(z); nh: out, then nhat
-    float2 d[4], yh[4], gt[4], nh[4], dn[4], wp[4], bp[4], sc[4];
+    float2 d[4], yh[4], gt[4], nh[4], dn[4];
     const float4 s4 = st;
     if (row + step < p.rows) st = __ldg(p.stats + row + step);
     auto read = [&](auto type, int slot, const void* src, int64_t from, float2(&o)[4]) {
@@ -532,13 +516,9 @@ __global__ void __launch_bounds__(kBound)
         yh[k] = mul2(add2(yh[k], bc2(-s4.x)), bc2(s4.y));
         gt[k] = make_float2(sigmoid_s(gt[k].x), sigmoid_s(gt[k].y));
       }
-      wps.get(wp, at);
-      bps.get(bp, at);
-      scs.get(sc, at);
     }
     if (next) {
-      float2 wq[4], a = bc2(0.f), b = bc2(0.f);
-      wqs.get(wq, at);
+      float2 a = bc2(0.f), b = bc2(0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (kPost) nh[k] = fma2(mul2(sc[k], gt[k]), fma2(yh[k], wp[k], bp[k]), nh[k]);
