@@ -22,16 +22,21 @@
 // the forward pass left at the tile's start (y in bf16 would cost dLambda three
 // digits), and the reverse recurrence uses the same products A.
 //
-// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 35 us, backward 79 us (and 3 for
+// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 33 us, backward 79 us (and 3 for
 // dLambda), where the bytes alone take 15 and 27 us at 6.5 TB/s; 1 x 32768 x 1024
-// forward 133 us (41). Neither memory bounds it (with all tiles read from the cache and
-// nothing stored the forward takes 34 us) nor the special functions (35 us without any)
-// nor one pipe (the fullest, FMA, is 46 % busy), but the phases of a tile between
-// barriers: 47 instructions an element at 0.57 a cycle and scheduler with 24 warps an
-// SM. Slower or the same: four CTAs an SM at 64 registers (40 us), every warp joining
-// the runs for itself (38 us), an mbarrier for each rank (39 us; the long prefill 198),
-// unpacked arithmetic (40 us), one reciprocal for both sigmoids (37 us); backward with
-// eight warps of eight steps (82 us) or two CTAs an SM at 64 registers (109 us).
+// forward 126 us (41): a round of the cluster takes 2.15 us with one CTA an SM, 3.1
+// with two and 4 with three, and clusters of 16 come to three on some SMs. Found at
+// 35.3 us, before the short form of slow decays: neither memory bounds the forward (with
+// all tiles read from the cache and nothing stored it took 34 us) nor the special
+// functions (35 us without any) nor one pipe (the fullest, FMA, 46 % busy), but the
+// phases of a tile between barriers: 47 instructions an element at 0.57 a cycle and
+// scheduler with 24 warps an SM. Slower or the same: four CTAs an SM at 64 registers
+// (40 us), every warp joining the runs for itself (38 us), an mbarrier for each rank
+// (39 us; the long prefill 198), bulk copies in place of st.async (36.7 us), unpacked
+// arithmetic (40 us), one reciprocal for both sigmoids (37 us), the next tile reduced
+// while the exchange is under way (one barrier a round, but two CTAs an SM: 46 us; the
+// long prefill 129 against 133); backward with eight warps of eight steps (82 us), two
+// CTAs an SM at 64 registers (109 us) or one joining warp of channel pairs (94 us).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -99,23 +104,27 @@ __device__ __forceinline__ float2 sigmoid2(float2 z) {
   return make_float2(rcp(d.x), rcp(d.y));
 }
 
-// exp(-l) - 1 for l >= 0: with -l = n ln 2 + f, |f| <= ln 2 / 2, it is
-// 2^n (e^f - 1) + (2^n - 1), e^f - 1 by its Taylor polynomial of degree 7
-// (remainder f^8 / 8!: below 2e-8 of f). Exact to the last place near l = 0 (n = 0),
-// where 1 - exp(-2 l) and the decay over many steps need it; for n < 0 the rounding of
-// n ln 2 adds 2e-8 n to f, less than 2^n / 4 of that to the result.
-__device__ __forceinline__ float2 expm1_neg2(float2 l) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
-  const float2 x = make_float2(max_nan(-l.x, -87.f), max_nan(-l.y, -87.f));
-  const float2 t = fma2(x, bc2(kLog2e), bc2(kMagic));
-  const float2 n = add2(t, bc2(-kMagic));
-  const float2 f = fma2(n, bc2(-0.693147180559945309f), x);
+// e^f - 1 for |f| <= kNear (just below ln 2 / 2, where n is 0 in the general form) by its Taylor polynomial of
+// degree 7 (remainder f^8 / 8!: below 2e-8 of f). Exact to the last place near 0, where
+// 1 - exp(-2 l) and the decay over many steps need it.
+constexpr float kNear = 0.3465f;
+__device__ __forceinline__ float2 expm1_near2(float2 f) {
   float2 p = fma2(f, bc2(1.f / 5040.f), bc2(1.f / 720.f));
   p = fma2(p, f, bc2(1.f / 120.f));
   p = fma2(p, f, bc2(1.f / 24.f));
   p = fma2(p, f, bc2(1.f / 6.f));
   p = fma2(p, f, bc2(0.5f));
-  p = fma2(mul2(p, f), f, f);
+  return fma2(mul2(p, f), f, f);
+}
+
+// e^v - 1 for v <= 0: with v = n ln 2 + f it is 2^n (e^f - 1) + (2^n - 1). For n < 0 the
+// rounding of n ln 2 adds 2e-8 n to f, less than 2^n / 4 of that to the result.
+__device__ __forceinline__ float2 expm1_neg2(float2 v) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
+  const float2 x = make_float2(max_nan(v.x, -87.f), max_nan(v.y, -87.f));
+  const float2 t = fma2(x, bc2(kLog2e), bc2(kMagic));
+  const float2 n = add2(t, bc2(-kMagic));
+  const float2 p = expm1_near2(fma2(n, bc2(-0.693147180559945309f), x));
   const float2 s = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
                                __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
   return fma2(s, p, add2(s, bc2(-1.f)));
@@ -125,10 +134,24 @@ __device__ __forceinline__ float softplus_acc(float u) {
   return u > 20.f ? u + log1pf(expf(-u)) : log1pf(expf(u));
 }
 
-// m = a - 1 and q = 1 - a^2 of a step with L = l.
-__device__ __forceinline__ void decay2(float2 l, float2& m, float2& q) {
-  m = expm1_neg2(l);
+// m = a - 1 and q = 1 - a^2 of a step with -L = v; kSmall: |v| <= kNear.
+template <bool kSmall>
+__device__ __forceinline__ void decay2(float2 v, float2& m, float2& q) {
+  m = kSmall ? expm1_near2(v) : expm1_neg2(v);
   q = mul2(neg2(m), add2(m, bc2(2.f)));
+}
+
+// -c softplus(Lambda) of two channels, 0 where there is none: what s(r) is multiplied
+// by to -L. As s(r) <= 1, a warp whose rates are all within kNear needs no reduction of
+// the exponent (small_rates; the bits are the same): decays of 0.7 a step and slower,
+// which is where such layers start and mostly stay. Forward, slow against fast decays:
+// 33.4 and 35.8 us at 4 x 2048 x 1536, 126 and 134 at 1 x 32768 x 1024. The backward
+// pass gains nothing from it (79.0 and 79.8) and has the general form alone.
+__device__ __forceinline__ float2 neg_rate2(float2 lam, float sharpness, bool ok0, bool ok1) {
+  return make_float2(ok0 ? -sharpness * softplus_acc(lam.x) : 0.f, ok1 ? -sharpness * softplus_acc(lam.y) : 0.f);
+}
+__device__ __forceinline__ bool small_rates(float2 nrate) {
+  return __all_sync(0xffffffffu, nrate.x >= -kNear && nrate.y >= -kNear);
 }
 
 // Products of decays are held as M = A - 1: (1 + M)(1 + m) - 1 = M + (M m + m). A
@@ -347,7 +370,8 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
   T* y = static_cast<T*>(p.y) + row0 * p.channels + c;
   const uint8_t* rst = kReset ? p.reset + row0 : nullptr;
   const float2 lam = load_f2(p.lambda, c, ok0, ok1);
-  const float2 rate = make_float2(p.sharpness * softplus_acc(lam.x), p.sharpness * softplus_acc(lam.y));
+  const float2 nrate = neg_rate2(lam, p.sharpness, ok0, ok1);
+  const bool small = small_rates(nrate);
   // the joining threads' channel and its state, passed from round to round
   const int jc = c0 + tid;
   const bool jok = tid < kChan && jc < p.channels;
@@ -376,13 +400,13 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f);
     // steps past the end keep the state; whole tiles do not look for it
-    auto reduce = [&](auto whole) {
+    auto reduce = [&](auto whole, auto slow) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
         const bool in = decltype(whole)::value || t0 + s < p.seq;
         float2 m, q;
-        decay2(mul2(rate, sigmoid2(unpack2(&sm.raw[1][row][2 * lane]))), m, q);
+        decay2<decltype(slow)::value>(mul2(nrate, sigmoid2(unpack2(&sm.raw[1][row][2 * lane]))), m, q);
         const float2 v =
             mul2(sigmoid2(unpack2(&sm.raw[2][row][2 * lane])), unpack2(&sm.raw[0][row][2 * lane]));
         u[s] = mul2(sqrt2(q), v);
@@ -399,8 +423,9 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
       }
     };
     const bool whole = (tile + 1) * kTile <= p.seq;
-    if (whole) reduce(std::true_type{});
-    else if (tile < tiles) reduce(std::false_type{});
+    if (whole && small) reduce(std::true_type{}, std::true_type{});
+    else if (whole) reduce(std::true_type{}, std::false_type{});
+    else if (tile < tiles) reduce(std::false_type{}, std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     __syncthreads();  // the runs are there, and the tile's rows are no longer read
     if (tile + csize < tiles) load(tile + csize);
@@ -488,7 +513,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
   const int64_t out0 = row0 * p.channels + c;
   const uint8_t* rst = kReset ? p.reset + row0 : nullptr;
   const float2 lam = load_f2(p.lambda, c, ok0, ok1);
-  const float2 rate = make_float2(p.sharpness * softplus_acc(lam.x), p.sharpness * softplus_acc(lam.y));
+  const float2 nrate = neg_rate2(lam, p.sharpness, ok0, ok1);
   // threads 0 .. 63 join the states, 64 .. 127 the gradients, one channel each
   const int jch = tid & (kChan - 1), jc = c0 + jch;
   const bool jok = tid < 2 * kChan && jc < p.channels;
@@ -537,7 +562,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
         float2 q;
         sr[s] = sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]));
         si[s] = sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane]));
-        decay2(mul2(rate, sr[s]), m[s], q);
+        decay2<false>(mul2(nrate, sr[s]), m[s], q);
         ib[s] = inv_sqrt2(q);
         drop[s] = kReset && in && rst[t0 + s] != 0;
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][row][2 * lane]));
@@ -620,7 +645,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
                                add2(bc2(1.f), neg2(si[s])));
         float2 ds = mul2(mul2(cc, term[s]), sr[s]);
         if (kReset && drop[s]) ds = bc2(0.f);
-        const float2 dr = mul2(mul2(ds, rate), add2(bc2(1.f), neg2(sr[s])));
+        const float2 dr = mul2(mul2(ds, nrate), add2(sr[s], bc2(-1.f)));
         if (decltype(whole)::value || t0 + s < p.seq) {
           dlam = add2(dlam, ds);
           const int64_t o = out0 + int64_t(t0 + s) * p.channels;
@@ -688,9 +713,9 @@ __global__ void __launch_bounds__(128)
   float* hb = h + b * channels + c;
   const float2 h0 = make_float2(hb[0], ok1 ? hb[1] : 0.f);
   const float2 lam = load_f2(lambda, c, true, ok1);
-  const float2 rate = make_float2(sharpness * softplus_acc(lam.x), sharpness * softplus_acc(lam.y));
+  const float2 nrate = neg_rate2(lam, sharpness, true, true);
   float2 m, q;
-  decay2(mul2(rate, sigmoid2(rv)), m, q);
+  decay2<false>(mul2(nrate, sigmoid2(rv)), m, q);
   const float2 u = mul2(sqrt2(q), mul2(sigmoid2(iv), xv));
   const float2 hn = fma2(add2(m, bc2(1.f)), h0, u);
   hb[0] = hn.x;
