@@ -540,7 +540,7 @@ MQC_API int mqc_probe_fp32_fma(float* out, int64_t iters, int64_t* fmas_per_laun
  * by the forward pass when not NULL, read by the backward pass. h0, hT, dhT, dh0
  * and dy may be NULL (zero, or not wanted). dlambda [channels] fp32.
  * The reference has no real-valued recurrence. */
-#define MQC_GATED_SCAN_TILE 64
+#define MQC_GATED_SCAN_TILE 32
 typedef struct mqc_gated_scan_args {
   int64_t batch, seq_len, channels;
   int32_t dtype;

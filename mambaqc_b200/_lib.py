@@ -84,7 +84,7 @@ class BcProjScanArgs(ctypes.Structure):
     ]
 
 
-MQC_GATED_SCAN_TILE = 64
+MQC_GATED_SCAN_TILE = 32
 
 
 class GatedScanArgs(ctypes.Structure):

@@ -60,7 +60,9 @@ using pk::mul2;
 using pk::neg2;
 
 constexpr int kChan = 64;  // channels of a CTA
-constexpr int kTile = MQC_GATED_SCAN_TILE;  // time steps of a tile
+constexpr int kTile = 64;  // time steps of a tile, forward
+constexpr int kBwdTile = MQC_GATED_SCAN_TILE;  // backward, and between two checkpoints
+static_assert(kTile % kBwdTile == 0, "checkpoints at the starts of runs");
 // CTAs of a cluster: as many as the exchange's shared memory leaves room for two CTAs
 // an SM beside (16 is the device's limit, above the portable 8)
 template <typename T>
@@ -213,12 +215,12 @@ __device__ __forceinline__ void store2(__nv_bfloat16* p, float2 o, bool ok0, boo
 // one copy moves (16 or 4: cp.async; else single elements through registers). Rows
 // from `rows` on and channels from `cols` on become zero and are not read. `src`: the
 // tile's first element, or NULL for zeros.
-template <typename T, int kBytes, int kThreads>
+template <typename T, int kBytes, int kThreads, int kRows>
 __device__ __forceinline__ void copy_tile(T* dst, const T* src, int64_t stride, int rows, int cols) {
   constexpr int kPer = kBytes / int(sizeof(T));  // elements a copy
   constexpr int kUnits = kChan / kPer;           // copies a row
-  constexpr int kEach = kTile * kUnits / kThreads;
-  static_assert(kTile * kUnits % kThreads == 0 && kThreads % kUnits == 0, "whole rounds");
+  constexpr int kEach = kRows * kUnits / kThreads;
+  static_assert(kRows * kUnits % kThreads == 0 && kThreads % kUnits == 0, "whole rounds");
   const int unit = int(threadIdx.x) % kUnits, row0 = int(threadIdx.x) / kUnits;
   const int c = unit * kPer;
   const int have = min(max(cols - c, 0), kPer) * int(sizeof(T));
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int c = c0 + 2 * lane;
   const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
-  const int tiles = (p.seq + kTile - 1) / kTile;
+  const int tiles = (p.seq + kTile - 1) / kTile, ckpts = (p.seq + kBwdTile - 1) / kBwdTile;
   const int64_t row0 = int64_t(b) * p.seq;
   const T* x = static_cast<const T*>(p.x) + row0 * p.xs + c0;
   const T* r = static_cast<const T*>(p.r) + row0 * p.rs + c0;
@@ -380,9 +382,9 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
   auto load = [&](int tile) {
     const int64_t t0 = int64_t(tile) * kTile;
     const int rows = p.seq - int(t0), cols = p.channels - c0;
-    copy_tile<T, kBytes, kThreads>(&sm.raw[0][0][0], x + t0 * p.xs, p.xs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[1][0][0], r + t0 * p.rs, p.rs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[2][0][0], iv + t0 * p.is, p.is, rows, cols);
+    copy_tile<T, kBytes, kThreads, kTile>(&sm.raw[0][0][0], x + t0 * p.xs, p.xs, rows, cols);
+    copy_tile<T, kBytes, kThreads, kTile>(&sm.raw[1][0][0], r + t0 * p.rs, p.rs, rows, cols);
+    copy_tile<T, kBytes, kThreads, kTile>(&sm.raw[2][0][0], iv + t0 * p.is, p.is, rows, cols);
   };
 
   if (csize > 1) exchange_init(&sm.ex);
@@ -448,11 +450,13 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
           carry = apply<kReset>(g.x, g.y, carry);
         }
       }
-      if (p.ckpt != nullptr && jok && tile < tiles)
-        p.ckpt[(int64_t(b) * tiles + tile) * p.channels + jc] = h;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         sm.start[w][tid] = h;
+        if (w * S % kBwdTile == 0) {
+          const int q = tile * (kTile / kBwdTile) + w * S / kBwdTile;
+          if (p.ckpt != nullptr && jok && q < ckpts) p.ckpt[(int64_t(b) * ckpts + q) * p.channels + jc] = h;
+        }
         const float2 g = sm.run[w][tid];
         h = apply<kReset>(g.x, g.y, h);
       }
@@ -478,11 +482,11 @@ __global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
 
 // ------------------------------------------------------------------ backward
 
-constexpr int kBwdWarps = 16;
+constexpr int kBwdWarps = 8;
 
 template <typename T>
 struct BwdSmem {
-  T raw[2][4][kTile][kChan];          // x, r, i, dy of this tile and the one before it
+  T raw[2][4][kBwdTile][kChan];          // x, r, i, dy of this tile and the one before it
   float2 run[kBwdWarps][kChan];       // (M, E) of each warp's run
   float back[kBwdWarps][kChan];       // G of each run: c before it = A c after it + G
   float start[kBwdWarps][kChan];      // state before each run
@@ -491,9 +495,9 @@ struct BwdSmem {
 };
 
 template <typename T, int kBytes, bool kVec, bool kReset>
-__global__ void __launch_bounds__(kBwdWarps * 32)
+__global__ void __launch_bounds__(kBwdWarps * 32, 2)
     gated_scan_bwd_kernel(const BwdArgs p) {
-  constexpr int W = kBwdWarps, S = kTile / W, kThreads = W * 32;
+  constexpr int W = kBwdWarps, S = kBwdTile / W, kThreads = W * 32;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   BwdSmem<T>& sm = *reinterpret_cast<BwdSmem<T>*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int c = c0 + 2 * lane;
   const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
-  const int tiles = (p.seq + kTile - 1) / kTile;
+  const int tiles = (p.seq + kBwdTile - 1) / kBwdTile;
   const int64_t row0 = int64_t(b) * p.seq;
   const T* x = static_cast<const T*>(p.x) + row0 * p.xs + c0;
   const T* r = static_cast<const T*>(p.r) + row0 * p.rs + c0;
@@ -521,17 +525,17 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
   float2 dlam = bc2(0.f);
 
   auto load = [&](int tile, int st) {
-    const int64_t t0 = int64_t(tile) * kTile;
+    const int64_t t0 = int64_t(tile) * kBwdTile;
     const int rows = p.seq - int(t0), cols = p.channels - c0;
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][0][0][0], x + t0 * p.xs, p.xs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][1][0][0], r + t0 * p.rs, p.rs, rows, cols);
-    copy_tile<T, kBytes, kThreads>(&sm.raw[st][2][0][0], iv + t0 * p.is, p.is, rows, cols);
+    copy_tile<T, kBytes, kThreads, kBwdTile>(&sm.raw[st][0][0][0], x + t0 * p.xs, p.xs, rows, cols);
+    copy_tile<T, kBytes, kThreads, kBwdTile>(&sm.raw[st][1][0][0], r + t0 * p.rs, p.rs, rows, cols);
+    copy_tile<T, kBytes, kThreads, kBwdTile>(&sm.raw[st][2][0][0], iv + t0 * p.is, p.is, rows, cols);
     if (dy != nullptr)
-      copy_tile<T, kBytes, kThreads>(&sm.raw[st][3][0][0], dy + t0 * p.dys, p.dys, rows, cols);
+      copy_tile<T, kBytes, kThreads, kBwdTile>(&sm.raw[st][3][0][0], dy + t0 * p.dys, p.dys, rows, cols);
   };
   if (dy == nullptr)
-    for (int k = tid; k < 2 * kTile * kChan; k += kThreads)
-      sm.raw[k / (kTile * kChan)][3][0][k % (kTile * kChan)] = T(0.f);
+    for (int k = tid; k < 2 * kBwdTile * kChan; k += kThreads)
+      sm.raw[k / (kBwdTile * kChan)][3][0][k % (kBwdTile * kChan)] = T(0.f);
 
   if (csize > 1) exchange_init(&sm.ex);
   // the cluster's tiles are taken from the end: rank 0 the last of each group
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
   int round = 0;
   for (int done = 0; done < tiles; done += csize, ++round) {
     const int tile = tiles - 1 - done - rank, st = round & 1;  // below 0: an empty tile
-    const int t0 = tile * kTile + warp * S;
+    const int t0 = tile * kBwdTile + warp * S;
     float h_tile = 0.f;
     if (jok && tid < kChan && tile >= 0)
       h_tile = p.ckpt[(int64_t(b) * tiles + tile) * p.channels + jc];
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32)
         G = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), g);
       }
     };
-    const bool here = tile >= 0, whole = here && (tile + 1) * kTile <= p.seq;
+    const bool here = tile >= 0, whole = here && (tile + 1) * kBwdTile <= p.seq;
     if (whole) reduce(std::true_type{});
     else if (here) reduce(std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
@@ -764,18 +768,26 @@ void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
   fit.known.store(1);
 }
 
+// What a round of a tile takes in a wave of clusters, in units of what each CTA that
+// shares the SM adds to it: `latency`, and the exchange between up to `few` CTAs or more.
+// Fitted to bf16 at nine shapes and cluster sizes 1 to 16; us at the sizes 1, 2, 4, 8:
+//   forward (units of 0.8 us)     4 x 2048 x 1536  62, 48, 35, -   64 x 512 x 1024  72, 81, 101, -
+//   backward (units of 0.88 us)   4 x 2048 x 1536  89, 82, 71, 75  64 x 512 x 1024  127, 154, 185, 255
+//                                 6 x 2048 x 1536  91, 83, 108, 111
+struct RoundCost {
+  double latency, exchange_few, exchange_more;
+  int few;
+};
+constexpr RoundCost kFwdCost = {1.5, 0.4, 1.6, 2};
+constexpr RoundCost kBwdCost = {0.5, 0.4, 0.9, 4};
+
 // Launches `units` clusters, one for each 64 channels of a sequence. The CTAs of a
 // cluster take consecutive tiles; of the sizes that fit (no more CTAs than tiles) it
 // is the one that takes the least time by a model of waves of clusters x rounds of a
-// tile x what a round takes: 1.5 for its latency, 1 for each CTA that shares the SM,
-// and `pair` for the exchange between two CTAs, `more` between more (forward 0.4 and 1.6
-// in units of 0.8 us; bf16, us: 4 x 2048 x 1536 with 1, 2, 4 CTAs 62, 48, 35; 6 x 2048 x
-// 1536 68, 50, 58; 64 x 512 x 1024 72, 81, 101; backward, whose rounds are longer, 0.5
-// and 0.75 in units of 1 us). *size: the size taken.
+// tile x RoundCost. *size: the size taken.
 template <auto kernel, typename A>
 int launch_clusters(const char* what, const A& args, int threads, size_t smem, int most,
-                    int64_t units, int tiles, double pair, double more, cudaStream_t st,
-                    int* size) {
+                    int64_t units, int tiles, const RoundCost& cost, cudaStream_t st, int* size) {
   static Fit fits[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -788,9 +800,9 @@ int launch_clusters(const char* what, const A& args, int threads, size_t smem, i
   for (int k = 0; k < kSizeCount && (c == 0 || kSizes[k] <= tiles); ++k) {
     const int64_t n = fit.clusters[k].load(), size = kSizes[k];
     if (n <= 0) continue;
-    const double exchange = size == 1 ? 0.0 : size == 2 ? pair : more;
+    const double exchange = size == 1 ? 0.0 : size <= cost.few ? cost.exchange_few : cost.exchange_more;
     auto wave = [&](int64_t u) {  // of u clusters
-      return u == 0 ? 0.0 : 1.5 + exchange + std::ceil(double(u * size) / sms);
+      return u == 0 ? 0.0 : cost.latency + exchange + std::ceil(double(u * size) / sms);
     };
     const double time = double((tiles + size - 1) / size) *
                         (double(units / n) * wave(n) + wave(units % n));
@@ -817,7 +829,7 @@ int run_fwd(const FwdArgs& f, cudaStream_t st) {
   int c;
   return launch_clusters<&gated_scan_fwd_kernel<T, kBytes, kVec, kReset>>(
       "mqc_gated_scan_fwd", f, kFwdWarps * 32, sizeof(FwdSmem<T>), kMaxCluster<T>,
-      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, 0.4, 1.6, st, &c);
+      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, kFwdCost, st, &c);
 }
 
 template <typename T, int kBytes, bool kVec, bool kReset>
@@ -825,7 +837,7 @@ int run_bwd(const BwdArgs& f, float* dlambda, cudaStream_t st) {
   int c = 0;
   if (int rc = launch_clusters<&gated_scan_bwd_kernel<T, kBytes, kVec, kReset>>(
           "mqc_gated_scan_bwd", f, kBwdWarps * 32, sizeof(BwdSmem<T>), kMaxCluster<T>,
-          int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, 0.5, 0.75, st, &c))
+          int64_t(f.batch) * f.chan_tiles, (f.seq + kBwdTile - 1) / kBwdTile, kBwdCost, st, &c))
     return rc;
   gated_scan_dlambda_kernel<<<(f.channels + 31) / 32, 256, 0, st>>>(
       f.part, f.lambda, dlambda, f.batch * c, f.channels, f.sharpness);
