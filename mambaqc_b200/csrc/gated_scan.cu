@@ -10,7 +10,7 @@
 //   dLambda = c s(Lambda) sum dL s(r)        dh0 = c[1]
 //
 // Layout. A CTA owns 64 channels of one sequence and walks over time in tiles of
-// kTile steps; each warp takes a run of consecutive steps of the tile, each lane
+// 32 or 64 steps; each warp takes a run of consecutive steps of the tile, each lane
 // two channels, so the arithmetic is packed two-wide; the tile's rows come through
 // shared memory (cp.async). A run is reduced to (A, E), h_out = A h_in + E (held as
 // A - 1), in registers; runs are joined through shared memory, tiles through the
@@ -22,7 +22,7 @@
 // the forward pass left at the tile's start (y in bf16 would cost dLambda three
 // digits), and the reverse recurrence uses the same products A.
 //
-// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 33 us, backward 79 us (and 3 for
+// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 34 us, backward 69 us (and 3 for
 // dLambda), where the bytes alone take 15 and 27 us at 6.5 TB/s; 1 x 32768 x 1024
 // forward 126 us (41): a round of the cluster takes 2.15 us with one CTA an SM, 3.1
 // with two and 4 with three, and clusters of 16 come to three on some SMs. Found at
@@ -35,8 +35,13 @@
 // (39 us; the long prefill 198), bulk copies in place of st.async (36.7 us), unpacked
 // arithmetic (40 us), one reciprocal for both sigmoids (37 us), the next tile reduced
 // while the exchange is under way (one barrier a round, but two CTAs an SM: 46 us; the
-// long prefill 129 against 133); backward with eight warps of eight steps (82 us), two
-// CTAs an SM at 64 registers (109 us) or one joining warp of channel pairs (94 us).
+// long prefill 129 against 133).
+//
+// Backward, tiles of 32 steps: the barriers of two CTAs an SM overlap, where one CTA of
+// 16 warps and tiles of 64 took 79 us (512 x 64 x 1024: 160 against 253). Slower: three
+// CTAs an SM at 85 registers (78 us); and with tiles of 64, eight warps of eight steps
+// (82 us), one joining warp of channel pairs (94 us), the states' half of the second
+// pass under the exchange for one more barrier (81 us; 64 x 512 x 1024 170 against 154).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -60,9 +65,14 @@ using pk::mul2;
 using pk::neg2;
 
 constexpr int kChan = 64;  // channels of a CTA
-constexpr int kTile = 64;  // time steps of a tile, forward
-constexpr int kBwdTile = MQC_GATED_SCAN_TILE;  // backward, and between two checkpoints
-static_assert(kTile % kBwdTile == 0, "checkpoints at the starts of runs");
+constexpr int kBwdTile = MQC_GATED_SCAN_TILE;  // time steps of a tile backward, and of a checkpoint
+constexpr int kRun = 8;  // steps of a warp's run forward
+// Forward, sequences of up to kShort steps go in tiles of 32 (four warps), longer ones
+// in tiles of 64 (eight). bf16, us with 32 and 64: 512 x 64 x 1024 66.5 and 86.2, 256 x
+// 128 x 1024 63 and 73, 64 x 512 x 1024 72 and 68, 4 x 2048 x 1536 33.3 and 34.2, 1 x
+// 32768 x 1024 147 and 127: small CTAs hide one another's loads where a sequence is done
+// in a round or two, large ones take half the rounds where it is long.
+constexpr int kShort = 128;
 // CTAs of a cluster: as many as the exchange's shared memory leaves room for two CTAs
 // an SM beside (16 is the device's limit, above the portable 8)
 template <typename T>
@@ -147,8 +157,8 @@ __device__ __forceinline__ void decay2(float2 v, float2& m, float2& q) {
 // by to -L. As s(r) <= 1, a warp whose rates are all within kNear needs no reduction of
 // the exponent (small_rates; the bits are the same): decays of 0.7 a step and slower,
 // which is where such layers start and mostly stay. Forward, slow against fast decays:
-// 33.4 and 35.8 us at 4 x 2048 x 1536, 126 and 134 at 1 x 32768 x 1024. The backward
-// pass gains nothing from it (79.0 and 79.8) and has the general form alone.
+// 33.6 and 35.8 us at 4 x 2048 x 1536, 126 and 134 at 1 x 32768 x 1024; backward 69 and
+// 70, 225 and 237.
 __device__ __forceinline__ float2 neg_rate2(float2 lam, float sharpness, bool ok0, bool ok1) {
   return make_float2(ok0 ? -sharpness * softplus_acc(lam.x) : 0.f, ok1 ? -sharpness * softplus_acc(lam.y) : 0.f);
 }
@@ -211,7 +221,7 @@ __device__ __forceinline__ void store2(__nv_bfloat16* p, float2 o, bool ok0, boo
   }
 }
 
-// One tile (kTile rows of kChan channels) of a tensor into shared memory. kBytes: what
+// One tile (kRows rows of kChan channels) of a tensor into shared memory. kBytes: what
 // one copy moves (16 or 4: cp.async; else single elements through registers). Rows
 // from `rows` on and channels from `cols` on become zero and are not read. `src`: the
 // tile's first element, or NULL for zeros.
@@ -336,13 +346,11 @@ __device__ __forceinline__ bool exchange(Exchange<kRanks>* x, int buf, uint32_t 
 
 // ------------------------------------------------------------------- forward
 
-constexpr int kFwdWarps = 8;
-
-template <typename T>
+template <typename T, int kWarps>
 struct FwdSmem {
-  T raw[3][kTile][kChan];             // x, r, i of a tile
-  float2 run[kFwdWarps][kChan];       // (M, E) of each warp's run
-  float start[kFwdWarps][kChan];      // state before each run
+  T raw[3][kWarps * kRun][kChan];      // x, r, i of a tile
+  float2 run[kWarps][kChan];          // (M, E) of each warp's run
+  float start[kWarps][kChan];         // state before each run
   Exchange<kMaxCluster<T>> ex;
 };
 
@@ -350,12 +358,13 @@ struct FwdSmem {
 // the runs, exchanges the tile's pair with the cluster and hands each run its start;
 // (C) each warp runs its steps again from there and stores y. The next tile's copies
 // are in flight from (B) on.
-template <typename T, int kBytes, bool kVec, bool kReset>
-__global__ void __launch_bounds__(kFwdWarps * 32, sizeof(T) == 2 ? 3 : 2)
+template <typename T, int kBytes, bool kVec, bool kReset, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWarps)
     gated_scan_fwd_kernel(const FwdArgs p) {
-  constexpr int W = kFwdWarps, S = kTile / W, kThreads = W * 32;
+  constexpr int W = kWarps, S = kRun, kThreads = W * 32, kTile = W * S;
+  static_assert(kTile % kBwdTile == 0 && kBwdTile % S == 0, "checkpoints at the starts of runs");
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  FwdSmem<T>& sm = *reinterpret_cast<FwdSmem<T>*>(smem_raw);
+  FwdSmem<T, W>& sm = *reinterpret_cast<FwdSmem<T, W>*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int csize = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int unit = int(blockIdx.x) / csize;
@@ -518,6 +527,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
   const uint8_t* rst = kReset ? p.reset + row0 : nullptr;
   const float2 lam = load_f2(p.lambda, c, ok0, ok1);
   const float2 nrate = neg_rate2(lam, p.sharpness, ok0, ok1);
+  const bool small = small_rates(nrate);
   // threads 0 .. 63 join the states, 64 .. 127 the gradients, one channel each
   const int jch = tid & (kChan - 1), jc = c0 + jch;
   const bool jok = tid < 2 * kChan && jc < p.channels;
@@ -558,7 +568,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f), G = bc2(0.f);
     // steps past the end pass c on (x and dy are 0 there); whole tiles do not look for it
-    auto reduce = [&](auto whole) {
+    auto reduce = [&](auto whole, auto slow) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
         float2 q;
         sr[s] = sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]));
         si[s] = sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane]));
-        decay2<false>(mul2(nrate, sr[s]), m[s], q);
+        decay2<decltype(slow)::value>(mul2(nrate, sr[s]), m[s], q);
         ib[s] = inv_sqrt2(q);
         drop[s] = kReset && in && rst[t0 + s] != 0;
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][row][2 * lane]));
@@ -586,8 +596,9 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
       }
     };
     const bool here = tile >= 0, whole = here && (tile + 1) * kBwdTile <= p.seq;
-    if (whole) reduce(std::true_type{});
-    else if (here) reduce(std::false_type{});
+    if (whole && small) reduce(std::true_type{}, std::true_type{});
+    else if (whole) reduce(std::true_type{}, std::false_type{});
+    else if (here) reduce(std::false_type{}, std::false_type{});
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     *reinterpret_cast<float2*>(&sm.back[warp][2 * lane]) = G;
     __syncthreads();
@@ -778,6 +789,7 @@ struct RoundCost {
   double latency, exchange_few, exchange_more;
   int few;
 };
+constexpr RoundCost kFwdShortCost = {1.9, 0.4, 1.5, 5};  // tiles of 32, units of 0.43 us
 constexpr RoundCost kFwdCost = {1.5, 0.4, 1.6, 2};
 constexpr RoundCost kBwdCost = {0.5, 0.4, 0.9, 4};
 
@@ -824,12 +836,18 @@ int launch_clusters(const char* what, const A& args, int threads, size_t smem, i
   return check_launch(what);
 }
 
+template <typename T, int kBytes, bool kVec, bool kReset, int kWarps>
+int run_fwd_tiles(const FwdArgs& f, const RoundCost& cost, cudaStream_t st) {
+  int c;
+  return launch_clusters<&gated_scan_fwd_kernel<T, kBytes, kVec, kReset, kWarps>>(
+      "mqc_gated_scan_fwd", f, kWarps * 32, sizeof(FwdSmem<T, kWarps>), kMaxCluster<T>,
+      int64_t(f.batch) * f.chan_tiles, (f.seq + kWarps * kRun - 1) / (kWarps * kRun), cost, st, &c);
+}
+
 template <typename T, int kBytes, bool kVec, bool kReset>
 int run_fwd(const FwdArgs& f, cudaStream_t st) {
-  int c;
-  return launch_clusters<&gated_scan_fwd_kernel<T, kBytes, kVec, kReset>>(
-      "mqc_gated_scan_fwd", f, kFwdWarps * 32, sizeof(FwdSmem<T>), kMaxCluster<T>,
-      int64_t(f.batch) * f.chan_tiles, (f.seq + kTile - 1) / kTile, kFwdCost, st, &c);
+  return f.seq <= kShort ? run_fwd_tiles<T, kBytes, kVec, kReset, 4>(f, kFwdShortCost, st)
+                         : run_fwd_tiles<T, kBytes, kVec, kReset, 8>(f, kFwdCost, st);
 }
 
 template <typename T, int kBytes, bool kVec, bool kReset>
@@ -852,7 +870,7 @@ int check_sizes(const char* what, const mqc_gated_scan_args* a) {
   MQC_REQUIRE(a->batch >= 0 && a->seq_len >= 0 && a->channels >= 0, MQC_ERR_INVALID_VALUE,
               "%s: batch %lld, seq_len %lld, channels %lld", what, (long long)a->batch,
               (long long)a->seq_len, (long long)a->channels);
-  MQC_REQUIRE(a->seq_len <= 0x7fffffff - 2 * kLargestCluster * kTile && a->channels <= 0x7fffffff - kChan &&
+  MQC_REQUIRE(a->seq_len <= 0x7fffffff - 2 * kLargestCluster * 64 && a->channels <= 0x7fffffff - kChan &&
                   a->batch <= 0x7fffffff / kLargestCluster,
               MQC_ERR_UNSUPPORTED, "%s: a size above 2^31", what);
   MQC_REQUIRE(a->sharpness > 0.f, MQC_ERR_INVALID_VALUE, "%s: sharpness %g", what,

@@ -49,7 +49,7 @@ def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda:
     document of a packed sequence): there h = s(i) x. Returns y [B, T, D] in x's
     dtype, and with ``return_final_state`` also h_T [B, D] fp32. The state is fp32
     throughout. Differentiable in x, r, i, Lambda, h0, from y and h_T; the backward
-    pass recomputes the states from fp32 ones kept every 64 steps (once: it has no
+    pass recomputes the states from fp32 ones kept every 32 steps (once: it has no
     second derivative)."""
     assert x.dim() == 3, f"x must be [B, T, D], got {tuple(x.shape)}"
     _check("gated_linear_scan", x, r, i, Lambda, h0)
