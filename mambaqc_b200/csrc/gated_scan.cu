@@ -24,7 +24,7 @@
 //
 // Measured, bf16, 4 x 2048 x 1536 on one B200: forward 34 us, backward 69 us (and 3 for
 // dLambda), where the bytes alone take 15 and 27 us at 6.5 TB/s; 1 x 32768 x 1024
-// forward 126 us (41): a round of the cluster takes 2.15 us with one CTA an SM, 3.1
+// forward 124 us (41): a round of the cluster takes 2.15 us with one CTA an SM, 3.1
 // with two and 4 with three, and clusters of 16 come to three on some SMs. Found at
 // 35.3 us, before the short form of slow decays: neither memory bounds the forward (with
 // all tiles read from the cache and nothing stored it took 34 us) nor the special
@@ -164,8 +164,8 @@ __device__ __forceinline__ void decay2(float2 v, float2& m, float2& q) {
 // by to -L. As s(r) <= 1, a warp whose rates are all within kNear needs no reduction of
 // the exponent (small_rates): decays of 0.7 a step and slower,
 // which is where such layers start and mostly stay. Forward, slow against fast decays:
-// 33.6 and 35.8 us at 4 x 2048 x 1536, 126 and 134 at 1 x 32768 x 1024; backward 69 and
-// 70, 225 and 237.
+// 33.7 and 35.8 us at 4 x 2048 x 1536, 124 and 134 at 1 x 32768 x 1024; backward 69 and
+// 70.8, 223 and 237.
 __device__ __forceinline__ float2 neg_rate2(float2 lam, float sharpness, bool ok0, bool ok1) {
   return make_float2(ok0 ? -sharpness * softplus_acc(lam.x) : 0.f, ok1 ? -sharpness * softplus_acc(lam.y) : 0.f);
 }

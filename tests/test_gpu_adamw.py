@@ -477,3 +477,15 @@ def test_refusals():
     sparse.grad = torch.sparse_coo_tensor([[1]], [[1.0, 1.0]], (4, 2)).to(DEV)
     with pytest.raises(RuntimeError, match="sparse"):
         AdamW([sparse]).step()
+
+
+def test_moments_have_the_bits_of_elementary_operations():
+    """No sum of products is fused: an 8-bit code follows from a moment's last bits."""
+    n = 100003
+    p, g, m, v = (torch.randn(n, generator=gen(k)).to(DEV) for k in range(4))
+    v = v.square()
+    want_m = m * 0.9 + g * (1 - 0.9)
+    want_v = v * 0.999 + (g * g) * (1 - 0.999)
+    adamw_step([p], [g], [m], [v], step=3, lr=1e-3, betas=(0.9, 0.999))
+    assert torch.equal(m, want_m)
+    assert torch.equal(v, want_v)
