@@ -181,14 +181,21 @@ __device__ __forceinline__ float2 join_decay(float2 M, float2 m) {
   return add2(M, fma2(M, m, m));
 }
 
-__device__ __forceinline__ float join_decay(float M, float m) { return M + fmaf(M, m, m); }
+// M of a run or tile with a reset in it. The state before it is dropped whatever else
+// the run holds, a NaN decay before or after the reset too; decays that multiply to
+// nothing (M = -1) drop nothing: a NaN state outlives them.
+constexpr float kDropped = -2.f;
 
-// A s + E with A = 1 + M. kDrop: where M is -1 (a reset) s is dropped, also if it is
-// infinite or NaN.
-template <bool kDrop>
+template <bool kReset>
+__device__ __forceinline__ float join_decay(float M, float m) {
+  return kReset && (M == kDropped || m == kDropped) ? kDropped : M + fmaf(M, m, m);
+}
+
+// A s + E with A = 1 + M.
+template <bool kReset>
 __device__ __forceinline__ float apply(float M, float E, float s) {
   const float r = s + fmaf(M, s, E);
-  return kDrop && M == -1.f ? E : r;
+  return kReset && M == kDropped ? E : r;
 }
 
 // sqrt(q), and 1 / sqrt(q) (1e19 at most: at q = 0 its product with q is 0, and what
@@ -417,6 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
     float2 a[S], u[S];
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f);
+    bool dropped = false;
     // steps past the end keep the state; whole tiles do not look for it
     auto reduce = [&](auto whole, auto slow) {
 #pragma unroll
@@ -433,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
         a[s] = add2(m, bc2(1.f));
         if (kReset && drop[s]) {
           u[s] = E = v;
-          M = bc2(-1.f);
+          dropped = true;
         } else {
           E = fma2(a[s], E, u[s]);
           M = join_decay(M, m);
@@ -444,6 +452,7 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
     if (whole && small) reduce(std::true_type{}, std::true_type{});
     else if (whole) reduce(std::true_type{}, std::false_type{});
     else if (tile < tiles) reduce(std::false_type{}, std::false_type{});
+    if (kReset && dropped) M = bc2(kDropped);
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     __syncthreads();  // the runs are there, and the tile's rows are no longer read
     if (tile + csize < tiles) load(tile + csize);
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
         for (int w = 0; w < W; ++w) {
           const float2 g = sm.run[w][tid];
           te = apply<kReset>(g.x, g.y, te);
-          tm = join_decay(tm, g.x);
+          tm = join_decay<kReset>(tm, g.x);
         }
         if (alive)
           alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, tm, te, p.status);
@@ -574,6 +583,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
     float2 m[S], sr[S], si[S], ib[S];
     bool drop[S];
     float2 M = bc2(0.f), E = bc2(0.f), G = bc2(0.f);
+    bool dropped = false;
     // steps past the end pass c on (x and dy are 0 there); whole tiles do not look for it
     auto reduce = [&](auto whole, auto slow) {
 #pragma unroll
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
         if (!in) m[s] = bc2(0.f);
         if (kReset && drop[s]) {
           E = v;
-          M = bc2(-1.f);
+          dropped = true;
         } else {
           E = fma2(add2(m[s], bc2(1.f)), E, mul2(mul2(q, ib[s]), v));
           M = join_decay(M, m[s]);
@@ -606,6 +616,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
     if (whole && small) reduce(std::true_type{}, std::true_type{});
     else if (whole) reduce(std::true_type{}, std::false_type{});
     else if (here) reduce(std::false_type{}, std::false_type{});
+    if (kReset && dropped) M = bc2(kDropped);
     *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
     *reinterpret_cast<float2*>(&sm.back[warp][2 * lane]) = G;
     __syncthreads();
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
         for (int w = W - 1; w >= 0; --w) {
           const float fm = sm.run[w][jch].x;
           tg = apply<kReset>(fm, sm.back[w][jch], tg);
-          tm = join_decay(tm, fm);
+          tm = join_decay<kReset>(tm, fm);
         }
         if (alive)
           alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, tm, tg, p.status);

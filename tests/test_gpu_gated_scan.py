@@ -347,3 +347,79 @@ def test_refusals():
         gated_linear_step(x[:, 0], r[:, 0], i[:, 0], lam, h0.bfloat16())
     with pytest.raises(AssertionError, match="out"):
         gated_linear_step(x[:, 0], r[:, 0], i[:, 0], lam, h0, out=h0[:1])
+
+
+# (batch, channels) whose sequences go one CTA each, and to clusters of CTAs
+ONE_CTA, CLUSTERS = (160, 256), (1, 8)
+
+
+@pytest.mark.parametrize("b,d", [ONE_CTA, CLUSTERS])
+@pytest.mark.parametrize("t_nan,t_reset", [(70, 100), (72, 75), (75, 72), (74, 74), (100, 70), (30, 190)])
+def test_reset_and_nan_in_one_tile(b, d, t_nan, t_reset):
+    """A NaN gate and a reset, in one run of steps or two runs of a tile: the NaN
+    reaches from its step to the next reset in y, and the gradients of the other
+    document and of other channels are those of clean inputs, bit for bit."""
+    t, ch = 200, 5
+    x, r, i, lam, h0, _ = _inputs(b, t, d, torch.float32, seed=4)
+    reset = torch.zeros(b, t, dtype=torch.bool)
+    reset[:, t_reset] = True
+
+    def run(gate):
+        leaves = [_dev(v).requires_grad_() for v in (x, gate, i, lam, h0)]
+        y, hT = gated_linear_scan(*leaves, _dev(reset), return_final_state=True)
+        return y.detach(), hT.detach(), torch.autograd.grad([y.sum() + hT.sum()], leaves)
+
+    y, hT, grads = run(r)
+    bad_r = r.clone()
+    bad_r[0, t_nan, ch] = math.nan
+    y2, hT2, grads2 = run(bad_r)
+    bad = torch.zeros(b, t, d, dtype=torch.bool, device=DEV)
+    last = t_reset if t_reset >= t_nan else t
+    bad[0, t_nan:last, ch] = True
+    assert torch.equal(torch.isnan(y2), bad)
+    assert torch.equal(y2[~bad], y[~bad])
+    assert torch.isnan(hT2).sum() == (t_reset < t_nan)
+    # the document without the NaN, in this channel; every other channel whole
+    clean = torch.ones(b, t, d, dtype=torch.bool, device=DEV)
+    clean[0, :, ch] = False
+    other = slice(t_reset, t) if t_nan < t_reset else slice(0, t_reset)
+    clean[0, other, ch] = True
+    if t_nan == t_reset:        # the step's own decay is not used at all
+        clean[:] = True
+        assert torch.isnan(grads2[1][0, t_nan, ch]) or grads2[1][0, t_nan, ch] == 0
+        clean[0, t_nan, ch] = False
+    for a, e in zip(grads2[:3], grads[:3]):
+        assert torch.equal(a[clean], e[clean])
+    keep = torch.arange(d, device=DEV) != ch
+    assert torch.equal(grads2[3][keep], grads[3][keep])
+    h0_clean = torch.ones(b, d, dtype=torch.bool, device=DEV)
+    h0_clean[0, ch] = t_nan >= t_reset
+    assert torch.equal(grads2[4][h0_clean], grads[4][h0_clean])
+
+
+@pytest.mark.parametrize("b,d", [ONE_CTA, CLUSTERS])
+def test_nan_outlives_vanishing_decays(b, d):
+    """Decays that multiply to nothing over a run are no reset: a NaN state stays one
+    in a call with ``reset``, and a call whose resets are all False has the bits of one
+    without."""
+    t = 200
+    x, r, i, _, h0, reset = _inputs(b, t, d, torch.float32, seed=6, resets=1e-9)
+    assert not reset.any()
+    for rate in (0.1, 2.0, 30.0):
+        lam = torch.log(torch.expm1(torch.full((d,), rate / C)))
+        h0 = h0.clone()
+        h0[0, 3] = math.nan
+        args = [_dev(v) for v in (x, r, i, lam, h0)]
+        y = gated_linear_scan(*args)
+        y2, hT = gated_linear_scan(*args, _dev(reset), return_final_state=True)
+        assert torch.isnan(y2[0, :, 3]).all() and torch.isnan(hT[0, 3]), rate
+        clean = torch.ones(b, t, d, dtype=torch.bool, device=DEV)
+        clean[0, :, 3] = False
+        assert torch.equal(y[clean], y2[clean])
+        # backward: a NaN that arrives from the end reaches the start
+        leaves = [v.clone().requires_grad_() for v in args[:4]] + [_dev(torch.zeros(b, d)).requires_grad_()]
+        _, hT = gated_linear_scan(*leaves, _dev(reset), return_final_state=True)
+        dhT = torch.ones_like(hT)
+        dhT[0, 3] = math.nan
+        dh0 = torch.autograd.grad(hT, leaves[4], dhT)[0]
+        assert torch.isnan(dh0[0, 3]) and torch.isnan(dh0).sum() == 1, rate
