@@ -90,11 +90,6 @@ __device__ __forceinline__ float rcp(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ float rsqrt_a(float v) {
-  float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float sqrt_a(float v) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -136,27 +131,36 @@ __device__ __forceinline__ float2 expm1_reduced2(float2 f) {
   return fma2(mul2(p, f), f, f);
 }
 
-// e^v - 1 for v <= 0: with v = n ln 2 + f it is 2^n (e^f - 1) + (2^n - 1). For n < 0 the
-// rounding of n ln 2 adds 2e-8 n to f, less than 2^n / 4 of that to the result.
-__device__ __forceinline__ float2 expm1_neg2(float2 v) {
+// a = e^v and m = e^v - 1 for v <= 0: with v = n ln 2 + f they are 2^n (e^f - 1) + 2^n and
+// 2^n (e^f - 1) + (2^n - 1), so a keeps its digits where it is small and m where it is.
+// The constant ln 2 is rounded: 2e-9 n in f. Below kLeast v counts as kLeast (a 1.6e-38):
+// n stays in the range of an exponent, and a above 0.
+constexpr float kLeast = -87.f;
+__device__ __forceinline__ void exp_neg2(float2 v, float2& a, float2& m) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
-  const float2 x = make_float2(max_nan(v.x, -87.f), max_nan(v.y, -87.f));
+  const float2 x = make_float2(max_nan(v.x, kLeast), max_nan(v.y, kLeast));
   const float2 t = fma2(x, bc2(kLog2e), bc2(kMagic));
   const float2 n = add2(t, bc2(-kMagic));
   const float2 p = expm1_reduced2(fma2(n, bc2(-0.693147180559945309f), x));
   const float2 s = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
                                __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
-  return fma2(s, p, add2(s, bc2(-1.f)));
+  a = fma2(s, p, s);
+  m = fma2(s, p, add2(s, bc2(-1.f)));
 }
 
 __device__ __forceinline__ float softplus_acc(float u) {
   return u > 20.f ? u + log1pf(expf(-u)) : log1pf(expf(u));
 }
 
-// m = a - 1 and q = 1 - a^2 of a step with -L = v; kSmall: |v| <= kNear.
+// a, m = a - 1 and q = 1 - a^2 = -m (m + 2) of a step with -L = v; kSmall: |v| <= kNear.
 template <bool kSmall>
-__device__ __forceinline__ void decay2(float2 v, float2& m, float2& q) {
-  m = kSmall ? expm1_near2(v) : expm1_neg2(v);
+__device__ __forceinline__ void decay2(float2 v, float2& a, float2& m, float2& q) {
+  if (kSmall) {
+    m = expm1_near2(v);
+    a = add2(m, bc2(1.f));
+  } else {
+    exp_neg2(v, a, m);
+  }
   q = mul2(neg2(m), add2(m, bc2(2.f)));
 }
 
@@ -173,37 +177,70 @@ __device__ __forceinline__ bool small_rates(float2 nrate) {
   return __all_sync(0xffffffffu, nrate.x >= -kNear && nrate.y >= -kNear);
 }
 
-// Products of decays are held as M = A - 1: (1 + M)(1 + m) - 1 = M + (M m + m). A
+// Products A of decays are held as M = A - 1: (1 + M)(1 + m) - 1 = M + (M m + m). A
 // product of fp32 numbers just below 1 loses j k 2^-48 each time, j and k their
 // distances from 1 in units of 2^-24, always to the same side; over a state's
-// memory of 1e4 steps that came to 4e-5 of it.
-__device__ __forceinline__ float2 join_decay(float2 M, float2 m) {
-  return add2(M, fma2(M, m, m));
+// memory of 1e4 steps that came to 4e-5 of it. M has 6e-8 of A at least, but only 6e-8:
+// under 1/2 it is A itself that counts, multiplied up beside M (where single decays are
+// above 0.7, 1 + M serves: 2e-6 of A over eight of them). A gradient carried as
+// s + (M s + E) over 32 steps of decay 0.6 was 25 % off.
+struct Product2 {
+  float2 M, A;
+};
+template <bool kSmall>
+__device__ __forceinline__ void join_step(Product2& t, float2 a, float2 m) {
+  t.M = add2(t.M, fma2(t.M, m, m));
+  if (!kSmall) t.A = mul2(t.A, a);
 }
 
-// M of a run or tile with a reset in it. The state before it is dropped whatever else
-// the run holds, a NaN decay before or after the reset too; decays that multiply to
-// nothing (M = -1) drop nothing: a NaN state outlives them.
+// The product of a run or a tile as one number: M (below 0) from A = 1/2 up, A (0 or
+// above) under that, and kDropped with a reset in the run. A product of exactly 1 is held
+// as -kTiny, which s + (M s + E) does not see.
 constexpr float kDropped = -2.f;
-
-template <bool kReset>
-__device__ __forceinline__ float join_decay(float M, float m) {
-  return kReset && (M == kDropped || m == kDropped) ? kDropped : M + fmaf(M, m, m);
+constexpr float kTiny = 1.17549435e-38f;
+__device__ __forceinline__ float product_of(float M, float A) {
+  return M >= -0.5f ? fminf(M, -kTiny) : A;
+}
+template <bool kSmall>
+__device__ __forceinline__ float2 product_of(const Product2& t) {
+  const float2 A = kSmall ? add2(t.M, bc2(1.f)) : t.A;
+  return make_float2(product_of(t.M.x, A.x), product_of(t.M.y, A.y));
 }
 
-// A s + E with A = 1 + M.
-template <bool kReset>
-__device__ __forceinline__ float apply(float M, float E, float s) {
-  const float r = s + fmaf(M, s, E);
-  return kReset && M == kDropped ? E : r;
+// The product of a tile's runs for one channel.
+template <bool kReset, int W>
+__device__ __forceinline__ float tile_product(const float2 (*run)[kChan], int ch) {
+  float M = 0.f, A = 1.f;
+  bool dropped = false;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float D = run[w][ch].x;
+    const float m = D < 0.f ? D : D - 1.f;
+    A *= D < 0.f ? D + 1.f : D;
+    M += fmaf(M, m, m);
+    dropped = dropped || (kReset && D == kDropped);
+  }
+  return dropped ? kDropped : product_of(M, A);
 }
 
-// sqrt(q), and 1 / sqrt(q) (1e19 at most: at q = 0 its product with q is 0, and what
-// else it multiplies is multiplied by L = 0 as well)
+// A s + E. A reset drops s whatever it is, a NaN decay in the same run notwithstanding;
+// decays that multiply to nothing drop no NaN. kInfinite: s may be infinite and stays
+// so, as every decay is above 0; without, the result is NaN there (the joins below look
+// for one and start again with kInfinite).
+template <bool kReset, bool kInfinite>
+__device__ __forceinline__ float apply(float D, float E, float s) {
+  // the factor of s, 1 or 0, and not s or 0: nothing else than two multiply-adds waits
+  // for s (a select there cost 4 % of the backward pass)
+  const float r = fmaf(D < 0.f ? 1.f : 0.f, s, fmaf(D, s, E));
+  if (kReset && D == kDropped) return E;
+  return kInfinite && fabsf(s) == __int_as_float(0x7f800000) ? s + E : r;
+}
+
 __device__ __forceinline__ float2 sqrt2(float2 q) { return make_float2(sqrt_a(q.x), sqrt_a(q.y)); }
-__device__ __forceinline__ float2 inv_sqrt2(float2 q) {
-  const float2 t = add2(q, bc2(1.17549435e-38f));
-  return make_float2(rsqrt_a(t.x), rsqrt_a(t.y));
+// 1 / beta (9e18 at most: at beta = 0 what it multiplies is multiplied by L = 0 as well)
+__device__ __forceinline__ float2 inv_beta2(float2 beta) {
+  const float2 t = add2(beta, bc2(1.0842022e-19f));
+  return make_float2(rcp(t.x), rcp(t.y));
 }
 
 // ------------------------------------------------------------------- memory
@@ -304,7 +341,7 @@ struct BwdArgs {
 // --------------------------------------------------- exchange between the CTAs
 
 // What one thread a channel of each CTA tells all CTAs of its cluster in a round: the
-// pair (M, E) of its tile, written into their shared memory with the bytes counted on
+// pair (D, E) of its tile, written into their shared memory with the bytes counted on
 // an mbarrier there, so a round needs no barrier of the cluster and no fence that
 // waits for the global stores in flight. Two buffers in turn: a CTA writes round k + 2
 // only after it has every message of round k + 1, which their senders sent after
@@ -363,12 +400,12 @@ __device__ __forceinline__ bool exchange(Exchange<kRanks>* x, int buf, uint32_t 
 template <typename T, int kWarps>
 struct FwdSmem {
   T raw[3][kWarps * kRun][kChan];      // x, r, i of a tile
-  float2 run[kWarps][kChan];          // (M, E) of each warp's run
+  float2 run[kWarps][kChan];          // (D, E) of each warp's run
   float start[kWarps][kChan];         // state before each run
   Exchange<kMaxCluster<T>> ex;
 };
 
-// One tile: (A) each warp reduces its run to (M, E); (B) one thread a channel joins
+// One tile: (A) each warp reduces its run to (D, E); (B) one thread a channel joins
 // the runs, exchanges the tile's pair with the cluster and hands each run its start;
 // (C) each warp runs its steps again from there and stores y. The next tile's copies
 // are in flight from (B) on.
@@ -423,69 +460,93 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
     __syncthreads();  // the tile has landed
     float2 a[S], u[S];
     bool drop[S];
-    float2 M = bc2(0.f), E = bc2(0.f);
-    bool dropped = false;
+    float2 D = bc2(-kTiny), E = bc2(0.f);
     // steps past the end keep the state; whole tiles do not look for it
     auto reduce = [&](auto whole, auto slow) {
+      Product2 t = {bc2(0.f), bc2(1.f)};
+      bool dropped = false;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
         const bool in = decltype(whole)::value || t0 + s < p.seq;
         float2 m, q;
-        decay2<decltype(slow)::value>(mul2(nrate, sigmoid2(unpack2(&sm.raw[1][row][2 * lane]))), m, q);
+        decay2<decltype(slow)::value>(mul2(nrate, sigmoid2(unpack2(&sm.raw[1][row][2 * lane]))), a[s], m, q);
         const float2 v =
             mul2(sigmoid2(unpack2(&sm.raw[2][row][2 * lane])), unpack2(&sm.raw[0][row][2 * lane]));
         u[s] = mul2(sqrt2(q), v);
         drop[s] = kReset && in && rst[t0 + s] != 0;
-        if (!in) m = u[s] = bc2(0.f);
-        a[s] = add2(m, bc2(1.f));
+        if (!in) {
+          m = u[s] = bc2(0.f);
+          a[s] = bc2(1.f);
+        }
         if (kReset && drop[s]) {
           u[s] = E = v;
           dropped = true;
         } else {
           E = fma2(a[s], E, u[s]);
-          M = join_decay(M, m);
+          join_step<decltype(slow)::value>(t, a[s], m);
         }
       }
+      D = kReset && dropped ? bc2(kDropped) : product_of<decltype(slow)::value>(t);
     };
     const bool whole = (tile + 1) * kTile <= p.seq;
     if (whole && small) reduce(std::true_type{}, std::true_type{});
     else if (whole) reduce(std::true_type{}, std::false_type{});
     else if (tile < tiles) reduce(std::false_type{}, std::false_type{});
-    if (kReset && dropped) M = bc2(kDropped);
-    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
+    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(D.x, E.x, D.y, E.y);
     __syncthreads();  // the runs are there, and the tile's rows are no longer read
     if (tile + csize < tiles) load(tile + csize);
     cp_async_commit();
     if (tid < kChan) {
-      float h = carry;
       if (csize > 1) {
-        float tm = 0.f, te = 0.f;
+        const float td = tile_product<kReset, W>(sm.run, tid);
+        auto total = [&](auto infinite) {
+          float te = 0.f;
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const float2 g = sm.run[w][tid];
+            te = apply<kReset, decltype(infinite)::value>(g.x, g.y, te);
+          }
+          return te;
+        };
+        float te = total(std::false_type{});
+        if (te != te) te = total(std::true_type{});
+        if (alive)
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, td, te, p.status);
+      }
+      // the carry over the round, and the state before each run; true: a state was
+      // infinite or NaN
+      float next;
+      auto place = [&](auto infinite) {
+        constexpr bool kInf = decltype(infinite)::value;
+        float h = carry, seen = 0.f;  // seen: 0 times the states
+        next = carry;
+        if (csize > 1) {
+          for (int k = 0; k < csize; ++k) {
+            if (k == rank) h = next;
+            const float2 g = sm.ex.sum[st][k][tid];
+            next = apply<kReset, kInf>(g.x, g.y, next);
+            if (kReset) seen = fmaf(next, 0.f, seen);
+          }
+          seen = fmaf(next, 0.f, seen);
+        }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
+          sm.start[w][tid] = h;
+          if (w * S % kBwdTile == 0) {
+            const int q = tile * (kTile / kBwdTile) + w * S / kBwdTile;
+            if (p.ckpt != nullptr && jok && q < ckpts) p.ckpt[(int64_t(b) * ckpts + q) * p.channels + jc] = h;
+          }
           const float2 g = sm.run[w][tid];
-          te = apply<kReset>(g.x, g.y, te);
-          tm = join_decay<kReset>(tm, g.x);
+          h = apply<kReset, kInf>(g.x, g.y, h);
+          if (kReset) seen = fmaf(h, 0.f, seen);
         }
-        if (alive)
-          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, tm, te, p.status);
-        for (int k = 0; k < csize; ++k) {
-          if (k == rank) h = carry;
-          const float2 g = sm.ex.sum[st][k][tid];
-          carry = apply<kReset>(g.x, g.y, carry);
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        sm.start[w][tid] = h;
-        if (w * S % kBwdTile == 0) {
-          const int q = tile * (kTile / kBwdTile) + w * S / kBwdTile;
-          if (p.ckpt != nullptr && jok && q < ckpts) p.ckpt[(int64_t(b) * ckpts + q) * p.channels + jc] = h;
-        }
-        const float2 g = sm.run[w][tid];
-        h = apply<kReset>(g.x, g.y, h);
-      }
-      if (csize == 1) carry = h;
+        seen = fmaf(h, 0.f, seen);
+        if (csize == 1) next = h;
+        return seen != seen;
+      };
+      if (place(std::false_type{})) place(std::true_type{});
+      carry = next;
     }
     __syncthreads();
     float2 h = *reinterpret_cast<const float2*>(&sm.start[warp][2 * lane]);
@@ -512,7 +573,7 @@ constexpr int kBwdWarps = 8;
 template <typename T>
 struct BwdSmem {
   T raw[2][4][kBwdTile][kChan];          // x, r, i, dy of this tile and the one before it
-  float2 run[kBwdWarps][kChan];       // (M, E) of each warp's run
+  float2 run[kBwdWarps][kChan];       // (D, E) of each warp's run
   float back[kBwdWarps][kChan];       // G of each run: c before it = A c after it + G
   float start[kBwdWarps][kChan];      // state before each run
   float after[kBwdWarps][kChan];      // c after each run
@@ -580,78 +641,115 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
     __syncthreads();  // the tile has landed; the other buffer is no longer read
     if (tile - csize >= 0) load(tile - csize, st ^ 1);
     cp_async_commit();
-    float2 m[S], sr[S], si[S], ib[S];
+    float2 a[S], sr[S], si[S], beta[S];
     bool drop[S];
-    float2 M = bc2(0.f), E = bc2(0.f), G = bc2(0.f);
-    bool dropped = false;
+    float2 D = bc2(-kTiny), E = bc2(0.f), G = bc2(0.f);
     // steps past the end pass c on (x and dy are 0 there); whole tiles do not look for it
     auto reduce = [&](auto whole, auto slow) {
+      Product2 t = {bc2(0.f), bc2(1.f)};
+      bool dropped = false;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int row = warp * S + s;
         const bool in = decltype(whole)::value || t0 + s < p.seq;
-        float2 q;
+        float2 m, q;
         sr[s] = sigmoid2(unpack2(&sm.raw[st][1][row][2 * lane]));
         si[s] = sigmoid2(unpack2(&sm.raw[st][2][row][2 * lane]));
-        decay2<decltype(slow)::value>(mul2(nrate, sr[s]), m[s], q);
-        ib[s] = inv_sqrt2(q);
+        decay2<decltype(slow)::value>(mul2(nrate, sr[s]), a[s], m, q);
+        beta[s] = sqrt2(q);
         drop[s] = kReset && in && rst[t0 + s] != 0;
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][row][2 * lane]));
-        if (!in) m[s] = bc2(0.f);
+        if (!in) {
+          m = bc2(0.f);
+          a[s] = bc2(1.f);
+        }
         if (kReset && drop[s]) {
           E = v;
           dropped = true;
         } else {
-          E = fma2(add2(m[s], bc2(1.f)), E, mul2(mul2(q, ib[s]), v));
-          M = join_decay(M, m[s]);
+          E = fma2(a[s], E, mul2(beta[s], v));
+          join_step<decltype(slow)::value>(t, a[s], m);
         }
       }
+      D = kReset && dropped ? bc2(kDropped) : product_of<decltype(slow)::value>(t);
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         const float2 g = add2(unpack2(&sm.raw[st][3][warp * S + s][2 * lane]), G);
-        G = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), g);
+        G = kReset && drop[s] ? bc2(0.f) : mul2(a[s], g);
       }
     };
     const bool here = tile >= 0, whole = here && (tile + 1) * kBwdTile <= p.seq;
     if (whole && small) reduce(std::true_type{}, std::true_type{});
     else if (whole) reduce(std::true_type{}, std::false_type{});
     else if (here) reduce(std::false_type{}, std::false_type{});
-    if (kReset && dropped) M = bc2(kDropped);
-    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(M.x, E.x, M.y, E.y);
+    *reinterpret_cast<float4*>(&sm.run[warp][2 * lane]) = make_float4(D.x, E.x, D.y, E.y);
     *reinterpret_cast<float2*>(&sm.back[warp][2 * lane]) = G;
     __syncthreads();
     if (tid < kChan) {
-      float h = h_tile;
+      auto place = [&](auto infinite) {
+        float h = h_tile, seen = 0.f;
+        float2 run[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) run[w] = sm.run[w][jch];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          sm.start[w][jch] = h;
+          h = apply<kReset, decltype(infinite)::value>(run[w].x, run[w].y, h);
+          if (kReset) seen = fmaf(h, 0.f, seen);
+        }
+        seen = fmaf(h, 0.f, seen);
+        return seen != seen;
+      };
+      if (place(std::false_type{})) place(std::true_type{});
+    } else if (tid < 2 * kChan) {
+      if (csize > 1) {
+        const float td = tile_product<kReset, W>(sm.run, jch);
+        auto total = [&](auto infinite) {
+          float tg = 0.f;
+#pragma unroll
+          for (int w = W - 1; w >= 0; --w)
+            tg = apply<kReset, decltype(infinite)::value>(sm.run[w][jch].x, sm.back[w][jch], tg);
+          return tg;
+        };
+        float tg = total(std::false_type{});
+        if (tg != tg) tg = total(std::true_type{});
+        if (alive)
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, td, tg, p.status);
+      }
+      // c over the round, and c after each run (loaded before, not between, the joins: 67.4
+      // us instead of 70 at 4 x 2048 x 1536; forward, with fewer registers, it is the reverse)
+      float next, D_of[W], G_of[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        sm.start[w][jch] = h;
-        const float2 g = sm.run[w][jch];
-        h = apply<kReset>(g.x, g.y, h);
+        D_of[w] = sm.run[w][jch].x;
+        G_of[w] = sm.back[w][jch];
       }
-    } else if (tid < 2 * kChan) {
-      float cc = carry;
-      if (csize > 1) {
-        float tm = 0.f, tg = 0.f;
+      auto place = [&](auto infinite) {
+        constexpr bool kInf = decltype(infinite)::value;
+        float cc = carry, seen = 0.f;
+        next = carry;
+        if (csize > 1) {
+#pragma unroll 4
+          for (int k = 0; k < csize; ++k) {
+            if (k == rank) cc = next;
+            const float2 g = sm.ex.sum[st][k][jch];
+            next = apply<kReset, kInf>(g.x, g.y, next);
+            if (kReset) seen = fmaf(next, 0.f, seen);
+          }
+          seen = fmaf(next, 0.f, seen);
+        }
 #pragma unroll
         for (int w = W - 1; w >= 0; --w) {
-          const float fm = sm.run[w][jch].x;
-          tg = apply<kReset>(fm, sm.back[w][jch], tg);
-          tm = join_decay<kReset>(tm, fm);
+          sm.after[w][jch] = cc;
+          cc = apply<kReset, kInf>(D_of[w], G_of[w], cc);
+          if (kReset) seen = fmaf(cc, 0.f, seen);
         }
-        if (alive)
-          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, tm, tg, p.status);
-        for (int k = 0; k < csize; ++k) {
-          if (k == rank) cc = carry;
-          const float2 g = sm.ex.sum[st][k][jch];
-          carry = apply<kReset>(g.x, g.y, carry);
-        }
-      }
-#pragma unroll
-      for (int w = W - 1; w >= 0; --w) {
-        sm.after[w][jch] = cc;
-        cc = apply<kReset>(sm.run[w][jch].x, sm.back[w][jch], cc);
-      }
-      if (csize == 1) carry = cc;
+        seen = fmaf(cc, 0.f, seen);
+        if (csize == 1) next = cc;
+        return seen != seen;
+      };
+      if (place(std::false_type{})) place(std::true_type{});
+      carry = next;
     }
     __syncthreads();
     // h[t-1] of each step forwards, then the gradients backwards
@@ -661,19 +759,17 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
       float2 term[S];  // a / beta s(i) x - h[t-1]: what c is multiplied by in dL
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const float2 a = add2(m[s], bc2(1.f));
-        const float2 beta = mul2(mul2(neg2(m[s]), add2(m[s], bc2(2.f))), ib[s]);
         const float2 v = mul2(si[s], unpack2(&sm.raw[st][0][warp * S + s][2 * lane]));
-        term[s] = fma2(mul2(a, ib[s]), v, neg2(h));
-        h = kReset && drop[s] ? v : fma2(a, h, mul2(beta, v));
-        ib[s] = kReset && drop[s] ? bc2(1.f) : beta;  // beta from here on
+        term[s] = fma2(mul2(a[s], inv_beta2(beta[s])), v, neg2(h));
+        h = kReset && drop[s] ? v : fma2(a[s], h, mul2(beta[s], v));
+        if (kReset && drop[s]) beta[s] = bc2(1.f);
       }
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         const int row = warp * S + s;
         const float2 gs = add2(unpack2(&sm.raw[st][3][row][2 * lane]), cc);
-        cc = kReset && drop[s] ? bc2(0.f) : mul2(add2(m[s], bc2(1.f)), gs);
-        const float2 dx = mul2(mul2(gs, ib[s]), si[s]);
+        cc = kReset && drop[s] ? bc2(0.f) : mul2(a[s], gs);
+        const float2 dx = mul2(mul2(gs, beta[s]), si[s]);
         const float2 di = mul2(mul2(dx, unpack2(&sm.raw[st][0][row][2 * lane])),
                                add2(bc2(1.f), neg2(si[s])));
         float2 ds = mul2(mul2(cc, term[s]), sr[s]);
@@ -747,10 +843,10 @@ __global__ void __launch_bounds__(128)
   const float2 h0 = make_float2(hb[0], ok1 ? hb[1] : 0.f);
   const float2 lam = load_f2(lambda, c, true, ok1);
   const float2 nrate = neg_rate2(lam, sharpness, true, true);
-  float2 m, q;
-  decay2<false>(mul2(nrate, sigmoid2(rv)), m, q);
+  float2 a, m, q;
+  decay2<false>(mul2(nrate, sigmoid2(rv)), a, m, q);
   const float2 u = mul2(sqrt2(q), mul2(sigmoid2(iv), xv));
-  const float2 hn = fma2(add2(m, bc2(1.f)), h0, u);
+  const float2 hn = fma2(a, h0, u);
   hb[0] = hn.x;
   if (ok1) hb[1] = hn.y;
   store2<kVec>(y + b * channels + c, hn, true, ok1);

@@ -423,3 +423,125 @@ def test_nan_outlives_vanishing_decays(b, d):
         dhT[0, 3] = math.nan
         dh0 = torch.autograd.grad(hT, leaves[4], dhT)[0]
         assert torch.isnan(dh0[0, 3]) and torch.isnan(dh0).sum() == 1, rate
+
+
+# Products of decays far from 1. Every step's -log a is a product of three fp32 factors:
+# the rate's softplus (log1pf and expf: 3 units of 6e-8), the sigmoid (its exponential's
+# argument and value, its reciprocal: 5) and two roundings; added up over the steps with
+# a rounding each, its relative error is below 1e-6. So a product exp(-S) is within
+# 1e-6 S of its value, and each of up to one join for every 8 steps rounds by 1e-7 more.
+def _decay_bound(total, steps):
+    return 1e-6 * total + 1e-7 * (steps / 8 + 10)
+
+
+@pytest.mark.parametrize("b,d", [ONE_CTA, CLUSTERS])
+@pytest.mark.parametrize("t", [1, 40, 200, 1500])
+@pytest.mark.parametrize("decay", [0.999, 0.9, 0.7, 0.6, 0.5, 0.1, 3e-7])
+def test_forgotten_state_keeps_its_digits(b, d, t, decay):
+    """With x = 0 the state is h0 times the product of the decays: each y and the last
+    state against 64 bits as long as fp32 has the value, and the gradient of h0 from the
+    last state alone, which is the product itself."""
+    if b > 1 and t > 200:
+        t = 300
+    g = gen(t)
+    rate = -math.log(decay)
+    lam = torch.full((d,), math.log(math.expm1(rate / C)))
+    r = 3.0 + torch.rand(b, t, d, generator=g)
+    x = torch.zeros(b, t, d)
+    h0 = 1e6 * (1 + torch.rand(b, d, generator=g))
+    leaf = _dev(h0).requires_grad_()
+    y, hT = gated_linear_scan(_dev(x), _dev(r), _dev(x), _dev(lam), leaf, return_final_state=True)
+    dh0 = torch.autograd.grad(hT.sum(), leaf)[0]
+    soft = torch.nn.functional.softplus(lam.to(DEV).double(), threshold=200.0)
+    total = torch.cumsum(C * soft * torch.sigmoid(r.to(DEV).double()), 1)
+    want = torch.exp(-total) * h0.to(DEV).double()[:, None]
+    steps = torch.arange(1, t + 1, device=DEV)[None, :, None]
+    bound = _decay_bound(total, steps)
+    held = want > 1e-30             # well inside fp32; below it only "next to nothing"
+    off = (y.double() - want).abs()
+    assert (off <= bound * want)[held].all(), (off / want / bound)[held].max()
+    assert (y.abs()[~held] <= 1.1e-30).all()
+    last = want[:, -1]
+    off = (hT.double() - last).abs()
+    assert torch.where(last > 1e-30, off <= bound[:, -1] * last, hT.abs() <= 1.1e-30).all()
+    last = torch.exp(-total[:, -1])
+    off = (dh0.double() - last).abs()
+    assert torch.where(last > 1e-30, off <= bound[:, -1] * last, dh0.abs() <= 1.1e-30).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 150, 64), (2, 700, 100), (160, 90, 256)])
+def test_gradients_under_fast_decay(shape):
+    """Rates up to 18 a step (decays down to 1e-8), a large start state, resets: every
+    channel's gradients against 64 bits. An error of 1e-6 of -log a is 1e-6 L of the
+    decay that dr, dLambda and the carried gradient are proportional to."""
+    b, t, d = shape
+    x, r, i, _, h0, reset = _inputs(b, t, d, torch.float32, seed=8, resets=0.02)
+    rates = torch.tensor([0.2, 1.0, 2.5, 5.0, 10.0, 15.0, 18.0, 30.0])[torch.arange(d) % 8]
+    lam = torch.where(rates / C > 0.1, torch.log(torch.expm1(rates / C)), torch.log(rates / C))
+    h0 = 1e4 * h0
+    g = gen(2)
+    dy, dhT = torch.randn(b, t, d, generator=g), torch.randn(b, d, generator=g)
+    out = []
+    for to in (lambda v: v.to(DEV), lambda v: v.to(DEV).double()):
+        leaves = [to(v).requires_grad_() for v in (x, r, i, lam, h0)]
+        f = gated_linear_scan if to(x).dtype == torch.float32 else None
+        if f is not None:
+            y, hT = f(*leaves, _dev(reset), return_final_state=True)
+        else:
+            y, hT = _ref(*leaves, _dev(reset))
+        out.append([y, hT, *torch.autograd.grad([y, hT], leaves, [to(dy), to(dhT)])])
+    soft = C * torch.nn.functional.softplus(lam.to(DEV).double(), threshold=200.0)
+    bound = 1e-5 + 2e-6 * soft
+    for name, got, want in zip(("y", "hT", "x", "r", "i", "Lambda", "h0"), *out):
+        got, want = got.double().reshape(-1, d), want.reshape(-1, d)
+        size = want.square().sum(0).sqrt()
+        off = (got - want).square().sum(0).sqrt()
+        # dLambda is one cancelling sum a channel, as in the test of slow decays: ten times
+        room = bound * size * (10 if name == "Lambda" else 1) + 1e-30
+        assert (off <= room).all(), (name, (off / room).max().item(), (off / room).argmax().item())
+
+
+@pytest.mark.parametrize("b,d", [ONE_CTA, CLUSTERS])
+@pytest.mark.parametrize("rate", [0.05, 0.9, 6.0, 18.0])
+@pytest.mark.parametrize("masked", [False, True])
+def test_infinite_states_stay_infinite(b, d, rate, masked):
+    """An infinite start state or input keeps its sign over runs and tiles, becomes NaN
+    where it meets the other infinity, and ends at a reset: the places of infinities
+    and NaN are those of 64 bits. An infinite gradient reaches the start state."""
+    t = 200
+    x, r, i, _, h0, _ = _inputs(b, t, d, torch.float32, seed=9)
+    lam = torch.log(torch.expm1(torch.full((d,), rate / C)))
+    h0[0, 0], h0[0, 1] = math.inf, -math.inf
+    x[0, 70, 2], x[0, 3, 3] = math.inf, -math.inf
+    x[0, 20, 4], x[0, 150, 4] = math.inf, -math.inf
+    reset = torch.zeros(b, t, dtype=torch.bool) if masked else None
+    if masked:
+        reset[:, 120] = True
+    leaf = _dev(h0).requires_grad_()
+    y, hT = gated_linear_scan(*map(_dev, (x, r, i, lam)), leaf, _dev(reset), return_final_state=True)
+    yr, hr = _ref(*(v.to(DEV).double() for v in (x, r, i, lam, h0)), _dev(reset))
+    for got, want in ((y, yr), (hT, hr)):
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.isposinf(got), torch.isposinf(want))
+        assert torch.equal(torch.isneginf(got), torch.isneginf(want))
+    dhT = torch.ones_like(hT)
+    dhT[0, 6], dhT[0, 7] = math.inf, -math.inf
+    dh0 = torch.autograd.grad(hT, leaf, dhT)[0]
+    if not masked:
+        assert torch.isposinf(dh0[0, 6]) and torch.isneginf(dh0[0, 7])
+        assert torch.isfinite(dh0).sum() == dh0.numel() - 2
+    else:
+        assert torch.count_nonzero(dh0) == 0
+
+
+@pytest.mark.parametrize("rate", [0.3, 2.0, 10.0, 15.0, 30.0])
+def test_step_keeps_the_digits_of_a_fast_decay(rate):
+    d = 37
+    lam = torch.log(torch.expm1(torch.full((d,), rate / C)))
+    r = torch.linspace(-2, 8, d)[None]
+    h0 = torch.full((1, d), 1e6)
+    h, zero = _dev(h0), torch.zeros(1, d, device=DEV)
+    gated_linear_step(zero, _dev(r), zero, _dev(lam), h)
+    total = C * torch.nn.functional.softplus(lam.double(), threshold=200.0) * torch.sigmoid(r.double())
+    want = 1e6 * torch.exp(-total)
+    assert ((h.cpu().double() / want - 1).abs() <= _decay_bound(total, 1)).all()
