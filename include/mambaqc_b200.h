@@ -554,6 +554,9 @@ typedef struct mqc_gated_scan_args {
   int64_t dy_row;
   void *dx, *dr, *di, *dlambda, *dh0;
   void* status; /* device int32 or NULL: a bounded wait that gave up */
+  /* The wait for a cluster's other CTAs gives up after about a second and reports to
+   * `status` (the results are then invalid). Not 0: at once. */
+  int32_t give_up, reserved0;
 } mqc_gated_scan_args;
 MQC_API int mqc_gated_scan_fwd(const mqc_gated_scan_args* args, void* stream);
 

@@ -99,7 +99,8 @@ class GatedScanArgs(ctypes.Structure):
         ("y", _c_void_p), ("hT", _c_void_p), ("ckpt", _c_void_p),
         ("dy", _c_void_p), ("dhT", _c_void_p), ("dy_row", _i64),
         ("dx", _c_void_p), ("dr", _c_void_p), ("di", _c_void_p), ("dlambda", _c_void_p),
-        ("dh0", _c_void_p), ("status", _c_void_p),
+        ("dh0", _c_void_p), ("status", _c_void_p), ("give_up", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
     ]
 
 

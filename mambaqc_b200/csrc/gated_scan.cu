@@ -319,6 +319,7 @@ struct FwdArgs {
   float* hT;
   float* ckpt;  // [batch][tiles][channels]: state before each tile, or NULL
   int* status;
+  int give_up;  // waits give up at once
   int batch, seq, channels, chan_tiles;
   float sharpness;
 };
@@ -334,6 +335,7 @@ struct BwdArgs {
   float* dh0;
   float* part;  // [batch][channels] x cluster rank: sums of dL s(r)
   int* status;
+  int give_up;  // waits give up at once
   int batch, seq, channels, chan_tiles;
   float sharpness;
 };
@@ -351,7 +353,10 @@ struct Exchange {
   float2 sum[2][kRanks][kChan];
   uint64_t bar[2];
 };
-constexpr int kPollLimit = 1 << 22;  // then the wait is given up and reported
+// A poll may sleep for up to kPollNs; after kPollLimit of them, about a second, a wait is
+// given up and reported.
+constexpr int kPollNs = 1000;
+constexpr int kPollLimit = 1 << 20;
 
 template <int kRanks>
 __device__ __forceinline__ void exchange_init(Exchange<kRanks>* x) {
@@ -368,30 +373,40 @@ __device__ __forceinline__ uint32_t remote_addr(uint32_t addr, int rank) {
   return r;
 }
 
-// Sends this channel's pair and waits for those of all ranks; false: given up.
+// Whether the round's messages are all here, after up to kPollLimit polls. (A limit
+// that is an argument costs the forward pass 3 to 5 % in registers.)
+__device__ __forceinline__ bool exchange_wait(uint32_t bar, uint32_t parity) {
+  for (int k = 0; k < kPollLimit; ++k) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "n"(kPollNs)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
+// Sends this channel's pair and waits for those of all ranks; false: given up (at once,
+// if asked to) and reported, after a second wait for the messages that are on their way
+// to this CTA (a channel whose wait was given up sends no more).
 template <int kRanks>
 __device__ __forceinline__ bool exchange(Exchange<kRanks>* x, int buf, uint32_t parity, int rank, int csize,
-                                         int ch, float m, float e, int* status) {
+                                         int ch, float d, float e, bool give_up, int* status) {
   if (ch == 0) mbar_arrive_expect_tx(&x->bar[buf], uint32_t(csize * kChan * sizeof(float2)));
   const uint32_t at = smem_addr(&x->sum[buf][rank][ch]), bar = smem_addr(&x->bar[buf]);
   for (int to = 0; to < csize; ++to)
     asm volatile(
         "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::
             "r"(remote_addr(at, to)),
-        "f"(m), "f"(e), "r"(remote_addr(bar, to))
+        "f"(d), "f"(e), "r"(remote_addr(bar, to))
         : "memory");
-  for (int k = 0; k < kPollLimit; ++k) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
+  if (!give_up && exchange_wait(bar, parity)) return true;
   report_status(status, MQC_DEVICE_STATUS_TIMEOUT);
+  exchange_wait(bar, parity);
   return false;
 }
 
@@ -512,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32, (sizeof(T) == 2 ? 24 : 16) / kWar
         float te = total(std::false_type{});
         if (te != te) te = total(std::true_type{});
         if (alive)
-          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, td, te, p.status);
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, tid, td, te, p.give_up != 0, p.status);
       }
       // the carry over the round, and the state before each run; true: a state was
       // infinite or NaN
@@ -714,7 +729,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2)
         float tg = total(std::false_type{});
         if (tg != tg) tg = total(std::true_type{});
         if (alive)
-          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, td, tg, p.status);
+          alive = exchange(&sm.ex, st, uint32_t(round >> 1) & 1u, rank, csize, jch, td, tg, p.give_up != 0, p.status);
       }
       // c over the round, and c after each run (loaded before, not between, the joins: 67.4
       // us instead of 70 at 4 x 2048 x 1536; forward, with fewer registers, it is the reverse)
@@ -1053,9 +1068,9 @@ int mqc_gated_scan_fwd(const mqc_gated_scan_args* a, void* stream) {
   FwdArgs f = {a->x, a->r, a->i, a->x_row, a->r_row, a->i_row,
                static_cast<const float*>(a->lambda_), static_cast<const float*>(a->h0),
                static_cast<const uint8_t*>(a->reset), a->y, static_cast<float*>(a->hT),
-               static_cast<float*>(a->ckpt), static_cast<int*>(a->status), int(a->batch),
-               int(a->seq_len), int(a->channels),
-               int((a->channels + kChan - 1) / kChan), a->sharpness};
+               static_cast<float*>(a->ckpt), static_cast<int*>(a->status), a->give_up, int(a->batch),
+               int(a->seq_len), int(a->channels), int((a->channels + kChan - 1) / kChan),
+               a->sharpness};
   const int bytes = copy_bytes(a->channels, es, {a->x, a->r, a->i}, {a->y},
                                {a->x_row, a->r_row, a->i_row});
   const bool rst = a->reset != nullptr;
@@ -1109,8 +1124,8 @@ int mqc_gated_scan_bwd(const mqc_gated_scan_args* a, void* workspace, size_t wor
                static_cast<const float*>(a->lambda_), static_cast<const uint8_t*>(a->reset),
                static_cast<const float*>(a->ckpt), static_cast<const float*>(a->dhT), a->dx, a->dr,
                a->di, static_cast<float*>(a->dh0), static_cast<float*>(workspace),
-               static_cast<int*>(a->status), int(a->batch), int(a->seq_len), int(a->channels), int((a->channels + kChan - 1) / kChan),
-               a->sharpness};
+               static_cast<int*>(a->status), a->give_up, int(a->batch), int(a->seq_len),
+               int(a->channels), int((a->channels + kChan - 1) / kChan), a->sharpness};
   float* dl = static_cast<float*>(a->dlambda);
   const int bytes = copy_bytes(a->channels, es, {a->x, a->r, a->i, a->dy}, {a->dx, a->dr, a->di},
                                {a->x_row, a->r_row, a->i_row, a->dy ? a->dy_row : 0});

@@ -14,6 +14,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <cstdlib>
+#include <cstring>
+
 #include "mambaqc_b200.h"
 
 namespace {
@@ -119,6 +122,22 @@ Tensor rows_of(const Tensor& t, int64_t width, int64_t* row) {
   return t.contiguous();
 }
 
+// Where each call is asked to check itself (MAMBAQC_B200_SYNC_CHECK=1): an error if a
+// kernel has reported a wait that it gave up to the status word of the tensor's device.
+void check_status(int64_t status, const Tensor& on) {
+  const char* wanted = std::getenv("MAMBAQC_B200_SYNC_CHECK");
+  if (wanted == nullptr || std::strcmp(wanted, "1") != 0) return;
+  at::NoGradGuard no_grad;
+  Tensor word = at::from_blob(reinterpret_cast<void*>(status), {1},
+                              on.options().dtype(at::kInt).requires_grad(false));
+  const int value = word.item<int>();
+  if (value == 0) return;
+  word.zero_();
+  if (value & MQC_DEVICE_STATUS_TIMEOUT)
+    throw std::runtime_error(
+        "mambaqc_b200: a bounded device-side wait timed out; results of that launch are invalid");
+}
+
 cudaStream_t stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
@@ -153,7 +172,8 @@ struct ScanInputs {
   int64_t x_row, r_row, i_row;
 };
 
-mqc_gated_scan_args scan_args(const ScanInputs& in, double sharpness, int64_t status) {
+mqc_gated_scan_args scan_args(const ScanInputs& in, double sharpness, int64_t status,
+                              bool give_up) {
   mqc_gated_scan_args a = {};
   a.batch = in.x.size(0);
   a.seq_len = in.x.size(1);
@@ -169,24 +189,26 @@ mqc_gated_scan_args scan_args(const ScanInputs& in, double sharpness, int64_t st
   a.lambda_ = ptr(in.lambda);
   a.reset = ptr(in.reset);
   a.status = reinterpret_cast<void*>(status);
+  a.give_up = give_up;
   return a;
 }
 
 // (y, hT, ckpt); hT and ckpt are undefined where they are not wanted.
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const ScanInputs& in, const Tensor& h0,
                                                 double sharpness, bool want_state, bool keep,
-                                                int64_t status) {
+                                                int64_t status, bool give_up) {
   c10::cuda::CUDAGuard guard(in.x.device());
   const int64_t b = in.x.size(0), t = in.x.size(1), d = in.x.size(2);
   Tensor y = like(in.x), hT, ckpt;
   if (want_state) hT = f32(in.x, {b, d});
   if (keep) ckpt = f32(in.x, {b, (t + MQC_GATED_SCAN_TILE - 1) / MQC_GATED_SCAN_TILE, d});
-  mqc_gated_scan_args a = scan_args(in, sharpness, status);
+  mqc_gated_scan_args a = scan_args(in, sharpness, status, give_up);
   a.h0 = ptr(h0);
   a.y = ptr(y);
   a.hT = ptr(hT);
   a.ckpt = ptr(ckpt);
   check(api.gated_scan_fwd(&a, stream_of(in.x)), "mqc_gated_scan_fwd");
+  check_status(status, in.x);
   return {y, hT, ckpt};
 }
 
@@ -206,13 +228,14 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& r,
                                const Tensor& i, const Tensor& lambda, const OptTensor& h0_,
                                const OptTensor& reset, double sharpness, bool want_state,
-                               int64_t status) {
+                               int64_t status, bool give_up) {
     const Tensor h0 = defined(h0_);
     const ScanInputs in = scan_inputs(x, r, i, lambda, defined(reset));
-    auto [y, hT, ckpt] = scan_forward(in, as_f32(h0), sharpness, want_state, true, status);
+    auto [y, hT, ckpt] = scan_forward(in, as_f32(h0), sharpness, want_state, true, status, give_up);
     ctx->save_for_backward({in.x, in.r, in.i, in.lambda, in.reset, ckpt});
     ctx->saved_data["sharpness"] = sharpness;
     ctx->saved_data["status"] = status;
+    if (give_up) ctx->saved_data["give_up"] = true;
     ctx->saved_data["lambda"] = int64_t(lambda.scalar_type());
     ctx->saved_data["h0"] = h0.defined() ? int64_t(h0.scalar_type()) : int64_t(-1);
     ctx->set_materialize_grads(false);
@@ -225,8 +248,9 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     c10::cuda::CUDAGuard guard(in.x.device());
     const int64_t b = in.x.size(0), t = in.x.size(1), d = in.x.size(2);
     const int64_t h0_type = ctx->saved_data["h0"].toInt();
-    mqc_gated_scan_args a =
-        scan_args(in, ctx->saved_data["sharpness"].toDouble(), ctx->saved_data["status"].toInt());
+    const int64_t status = ctx->saved_data["status"].toInt();
+    mqc_gated_scan_args a = scan_args(in, ctx->saved_data["sharpness"].toDouble(), status,
+                                      ctx->saved_data.count("give_up") != 0);
     a.ckpt = ptr(saved[5]);
     a.dy_row = d;
     Tensor dy;
@@ -245,25 +269,27 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     a.dlambda = ptr(dlambda);
     a.dh0 = ptr(dh0);
     check(api.gated_scan_bwd(&a, ptr(ws), bytes, stream_of(in.x)), "mqc_gated_scan_bwd");
+    check_status(status, in.x);
     dlambda = as_type(dlambda, at::ScalarType(ctx->saved_data["lambda"].toInt()));
     if (dh0.defined()) dh0 = as_type(dh0, at::ScalarType(h0_type));
-    return once({dx, dr, di, dlambda, dh0, Tensor(), Tensor(), Tensor(), Tensor()}, grads);
+    return once({dx, dr, di, dlambda, dh0, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, grads);
   }
 };
 
 std::tuple<Tensor, OptTensor> gated_scan(const Tensor& x, const Tensor& r, const Tensor& i,
                                          const Tensor& lambda, const OptTensor& h0,
                                          const OptTensor& reset, double sharpness, bool want_state,
-                                         int64_t status) {
+                                         int64_t status, bool give_up) {
   const Tensor h = defined(h0), rst = defined(reset);
   if (at::GradMode::is_enabled() && (x.requires_grad() || r.requires_grad() || i.requires_grad() ||
                                      lambda.requires_grad() || wants_grad(h))) {
-    variable_list out = GatedScan::apply(x, r, i, lambda, h0, reset, sharpness, want_state, status);
+    variable_list out =
+        GatedScan::apply(x, r, i, lambda, h0, reset, sharpness, want_state, status, give_up);
     return {out[0], want_state ? OptTensor(out[1]) : OptTensor()};
   }
   at::NoGradGuard no_grad;
-  auto [y, hT, ckpt] =
-      scan_forward(scan_inputs(x, r, i, lambda, rst), as_f32(h), sharpness, want_state, false, status);
+  auto [y, hT, ckpt] = scan_forward(scan_inputs(x, r, i, lambda, rst), as_f32(h), sharpness,
+                                    want_state, false, status, give_up);
   return {y, want_state ? OptTensor(hT) : OptTensor()};
 }
 

@@ -40,7 +40,8 @@ def _check(what, x, r, i, Lambda, h):
 
 def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda: torch.Tensor,
                       h0: torch.Tensor | None = None, reset: torch.Tensor | None = None, *,
-                      sharpness: float = 8.0, return_final_state: bool = False):
+                      sharpness: float = 8.0, return_final_state: bool = False,
+                      wait_poll_limit: int = -1):
     """The recurrence over x, r, i [B, T, D] (fp32 or bf16, one dtype; the recurrence
     and input gates r and i before their sigmoid; column slices of wider tensors are
     read in place), Lambda [D], start state h0 [B, D] (zero if None).
@@ -50,16 +51,23 @@ def gated_linear_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, Lambda:
     dtype, and with ``return_final_state`` also h_T [B, D] fp32. The state is fp32
     throughout. Differentiable in x, r, i, Lambda, h0, from y and h_T; the backward
     pass recomputes the states from fp32 ones kept every 32 steps (once: it has no
-    second derivative)."""
+    second derivative).
+
+    A device-side wait, forward or backward, that is not over after about a second gives up
+    and reports to the device's status word, which ``_lib.check_device_status`` turns into
+    an error, and each call by itself where MAMBAQC_B200_SYNC_CHECK is 1.
+    ``wait_poll_limit`` 0 makes it give up at once (for tests)."""
     assert x.dim() == 3, f"x must be [B, T, D], got {tuple(x.shape)}"
     _check("gated_linear_scan", x, r, i, Lambda, h0)
     assert sharpness > 0, "sharpness must be positive"
+    assert wait_poll_limit in (-1, 0), "wait_poll_limit must be -1 (default) or 0"
     if reset is not None:
         assert reset.dtype == torch.bool and reset.shape == x.shape[:2], \
             "reset must be bool [B, T]"
         assert reset.device == x.device, "gated_linear_scan: tensors on different devices"
     y, hT = _lib.torch_ops().gated_scan(x, r, i, Lambda, h0, reset, float(sharpness),
-                                        return_final_state, _lib.status_ptr(x.get_device()))
+                                        return_final_state, _lib.status_ptr(x.get_device()),
+                                        wait_poll_limit == 0)
     return (y, hT) if return_final_state else y
 
 

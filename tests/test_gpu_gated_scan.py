@@ -16,6 +16,7 @@ from tests.gpu_util import DEV, RTOL_F32, gen, rel_l2
 
 pytestmark = pytest.mark.gpu
 
+from mambaqc_b200 import _lib  # noqa: E402
 from mambaqc_b200.kernels import gated_linear_scan, gated_linear_step  # noqa: E402
 
 TOL_BF16 = 2.0 ** -8 + 1e-5
@@ -545,3 +546,45 @@ def test_step_keeps_the_digits_of_a_fast_decay(rate):
     total = C * torch.nn.functional.softplus(lam.double(), threshold=200.0) * torch.sigmoid(r.double())
     want = 1e6 * torch.exp(-total)
     assert ((h.cpu().double() / want - 1).abs() <= _decay_bound(total, 1)).all()
+
+
+def test_device_timeout_is_reported_and_context_survives(monkeypatch):
+    """A wait for the cluster's other CTAs that is made to give up (no polls) reports to
+    the status word, forward and backward, and each call raises by itself under
+    MAMBAQC_B200_SYNC_CHECK=1; calls after it are right."""
+    monkeypatch.delenv("MAMBAQC_B200_SYNC_CHECK", raising=False)
+    x, r, i, lam, h0, _ = _inputs(1, 300, 8, torch.float32)     # one sequence: a cluster
+    dev = torch.device(DEV)
+    _lib.check_device_status(dev)
+    leaves = [_dev(v).requires_grad_() for v in (x, r, i, lam, h0)]
+
+    def scan(**kw):
+        return gated_linear_scan(*leaves, **kw)
+
+    y = scan(wait_poll_limit=0)
+    with pytest.raises(RuntimeError, match="timed out"):
+        _lib.check_device_status(dev)
+    torch.autograd.grad(y.sum(), leaves)
+    with pytest.raises(RuntimeError, match="timed out"):
+        _lib.check_device_status(dev)
+    late = scan(wait_poll_limit=0)
+    with pytest.raises(RuntimeError, match="timed out"):
+        _lib.check_device_status(dev)
+    monkeypatch.setenv("MAMBAQC_B200_SYNC_CHECK", "1")
+    with pytest.raises(RuntimeError, match="timed out"):
+        torch.autograd.grad(late.sum(), leaves)
+    with pytest.raises(RuntimeError, match="timed out"):
+        scan(wait_poll_limit=0)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="timed out"):
+        scan(wait_poll_limit=0)
+    with pytest.raises(AssertionError, match="wait_poll_limit"):
+        scan(wait_poll_limit=7)
+    y = scan()                                                  # the check itself passes
+    grads = torch.autograd.grad(y.sum(), leaves)
+    ref = [v.double().requires_grad_() for v in (x, r, i, lam, h0)]
+    yr, _ = _ref(*ref)
+    want = torch.autograd.grad(yr.sum(), ref)
+    assert rel_l2(y, yr) < RTOL_F32
+    for a, e in zip(grads, want):
+        assert rel_l2(a, e) < 10 * RTOL_F32
+    _lib.check_device_status(dev)
