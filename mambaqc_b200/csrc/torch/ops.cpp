@@ -88,6 +88,15 @@ T* ptr(const Tensor& t) {
 Tensor defined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// The operators have no forward-mode derivative: an input that carries a tangent is
+// refused, where reading its value alone would make the derivative vanish.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what,
+                ": forward-mode derivatives are not supported");
+}
+
 // Contiguous fp32 (the tensor itself where it is that already).
 Tensor as_f32(const Tensor& t) {
   if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous())) return t;
@@ -281,6 +290,7 @@ std::tuple<Tensor, OptTensor> gated_scan(const Tensor& x, const Tensor& r, const
                                          const OptTensor& reset, double sharpness, bool want_state,
                                          int64_t status, bool give_up) {
   const Tensor h = defined(h0), rst = defined(reset);
+  refuse_tangents("gated_linear_scan", {&x, &r, &i, &lambda, &h});
   if (at::GradMode::is_enabled() && (x.requires_grad() || r.requires_grad() || i.requires_grad() ||
                                      lambda.requires_grad() || wants_grad(h))) {
     variable_list out =
@@ -295,6 +305,7 @@ std::tuple<Tensor, OptTensor> gated_scan(const Tensor& x, const Tensor& r, const
 
 Tensor gated_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lambda,
                   const Tensor& h, double sharpness, const OptTensor& out) {
+  refuse_tangents("gated_linear_step", {&x, &r, &i, &lambda, &h});
   at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t d = x.size(1);
@@ -460,6 +471,8 @@ std::tuple<OptTensor, OptTensor> norm_gate(const Tensor& x, const OptTensor& y, 
   const at::ScalarType branch = branch_f32 ? at::kFloat : at::kBFloat16;
   const Tensor t[7] = {defined(y),     defined(z),           defined(weight),   defined(bias),
                        defined(scale), defined(next_weight), defined(next_bias)};
+  refuse_tangents(t[0].defined() ? "norm_gate_residual" : "residual_norm",
+                  {&x, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6]});
   bool grad = x.requires_grad();
   for (const Tensor& v : t) grad = grad || wants_grad(v);
   if (at::GradMode::is_enabled() && grad) {

@@ -588,3 +588,25 @@ def test_device_timeout_is_reported_and_context_survives(monkeypatch):
     for a, e in zip(grads, want):
         assert rel_l2(a, e) < 10 * RTOL_F32
     _lib.check_device_status(dev)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent must not vanish without a word: the operator has no forward mode."""
+    import torch.autograd.forward_ad as fwad
+    x, r, i, lam, h0, _ = map(_dev, _inputs(2, 6, 8, torch.float32))
+    for k in range(5):
+        for needs in (False, True):
+            with fwad.dual_level():
+                args = [x, r, i, lam, h0]
+                if needs:
+                    args[0] = x.clone().requires_grad_()
+                args[k] = fwad.make_dual(args[k], torch.ones_like(args[k]))
+                with pytest.raises(RuntimeError, match="forward"):
+                    gated_linear_scan(*args, return_final_state=True)
+                if k < 4 and not needs:
+                    with pytest.raises(RuntimeError, match="forward"):
+                        step = [x[:, 0], r[:, 0], i[:, 0], lam]
+                        step[k] = fwad.make_dual(step[k], torch.ones_like(step[k]))
+                        gated_linear_step(*step, h0.clone())
+    # outside a level nothing changes
+    assert torch.isfinite(gated_linear_scan(x, r, i, lam, h0)).all()

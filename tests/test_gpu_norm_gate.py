@@ -345,3 +345,23 @@ def test_refusals():
         residual_norm(wide, one)
     with pytest.raises(AssertionError, match="dtype"):
         residual_norm(q["x"], q["weight"], dtype=torch.float16)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent must not vanish without a word: the operators have no forward mode."""
+    import torch.autograd.forward_ad as fwad
+    q = {k: v.to(DEV) for k, v in _inputs(4, 16, F32, F32, True, True).items()}
+    for name in q:
+        for needs in (False, True):
+            with fwad.dual_level():
+                args = dict(q)
+                if needs:
+                    args["x"] = q["x"].clone().requires_grad_()
+                args[name] = fwad.make_dual(args[name], torch.ones_like(args[name]))
+                with pytest.raises(RuntimeError, match="forward"):
+                    _call(args, "rms")
+    with fwad.dual_level():
+        dual = fwad.make_dual(q["x"], torch.ones_like(q["x"]))
+        with pytest.raises(RuntimeError, match="forward"):
+            residual_norm(dual, q["weight"])
+    assert torch.isfinite(residual_norm(q["x"], q["weight"])).all()
