@@ -88,6 +88,12 @@ T* ptr(const Tensor& t) {
 Tensor defined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Counts a write in place by a kernel, so that autograd refuses a graph that saved what
+// was there before. (Tensors of inference mode have no count.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The operators have no forward-mode derivative: an input that carries a tangent is
 // refused, where reading its value alone would make the derivative vanish.
 void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
@@ -316,6 +322,8 @@ Tensor gated_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tenso
   check(api.gated_scan_step(ptr(xs), x_row, ptr(rs), r_row, ptr(is), i_row, ptr(lam), ptr(h), ptr(y),
                             x.size(0), d, float(sharpness), dtype_of(x), stream_of(x)),
         "mqc_gated_scan_step");
+  written(h);
+  if (out.has_value()) written(y);
   return y;
 }
 
@@ -608,6 +616,8 @@ void adamw_step(const List& params, const List& grads, const List& m, const List
     a.seed = uint32_t(seed);
     check(api.adamw_step(&a, stream_of(params[0])), "mqc_adamw_step");
   }
+  for (const List* list : {&params, &m, &v, &em, &ev})
+    for (const Tensor& t : *list) written(t);
 }
 
 std::tuple<List, List> adamw_moments(const List& m, const List& v, const List& em, const List& ev) {

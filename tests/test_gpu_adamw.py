@@ -489,3 +489,20 @@ def test_moments_have_the_bits_of_elementary_operations():
     adamw_step([p], [g], [m], [v], step=3, lr=1e-3, betas=(0.9, 0.999))
     assert torch.equal(m, want_m)
     assert torch.equal(v, want_v)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_step_advances_the_version_counters(bits):
+    """What a step writes in place counts as written: a second backward through a graph
+    from before the step raises instead of using the new weights."""
+    p = torch.nn.Parameter(torch.randn(300, generator=gen(1)).to(DEV))
+    opt = AdamW([p], lr=1e-2, state_bits=bits)
+    loss = p.square().sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    states = [v for v in opt.state[p].values() if torch.is_tensor(v)]
+    before = [v._version for v in (p, *states)]
+    opt.step(max_grad_norm=1.0)
+    assert [v._version for v in (p, *states)] == [k + 1 for k in before]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -610,3 +610,22 @@ def test_forward_mode_derivatives_are_refused():
                         gated_linear_step(*step, h0.clone())
     # outside a level nothing changes
     assert torch.isfinite(gated_linear_scan(x, r, i, lam, h0)).all()
+
+
+def test_step_advances_the_version_counters():
+    """A backward through a graph that saved the state before a step raises, as after
+    torch's own operations in place."""
+    x, r, i, lam, h0, _ = map(_dev, _inputs(2, 1, 8, torch.float32))
+    x, r, i = x[:, 0], r[:, 0], i[:, 0]
+    w = torch.ones_like(h0, requires_grad=True)
+    out = torch.empty_like(x)
+    loss = (w * h0).sum() + (w * out).sum()
+    before = h0._version, out._version, x._version
+    gated_linear_step(x, r, i, lam, h0, out=out)
+    assert (h0._version, out._version, x._version) == (before[0] + 1, before[1] + 1, before[2])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                    # states of inference mode have no count
+        state = h0.clone()
+        gated_linear_step(x.detach(), r, i, lam, state)
+    gated_linear_step(x, r, i, lam, state)
