@@ -29,7 +29,9 @@ class AdamW(torch.optim.Optimizer):
     max_grad_norm=...)`` clips by the global norm of all gradients without rewriting
     them and leaves the norm, a device scalar, in ``grad_norm``. A gradient that is
     infinite or NaN makes the moments and parameters NaN, as it would in 32 bits; in
-    8 bits it takes its block of 256 with it at the next step."""
+    8 bits it takes its block of 256 with it at the next step. One whose square is
+    infinite in fp32 (above 1.8e19) makes v infinite: the parameter takes no step from
+    it, and in 8 bits, where that marks the block, the block is NaN at the next step."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,

@@ -506,3 +506,69 @@ def test_step_advances_the_version_counters(bits):
     assert [v._version for v in (p, *states)] == [k + 1 for k in before]
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("pt", [F32, BF16])
+@pytest.mark.parametrize("size", [3e19, 1e25, 3e38])
+def test_finite_gradient_whose_square_overflows(bits, pt, size):
+    """v is infinite, so the update is m over infinity, nothing: the parameter moves by
+    its decay alone, as in the formula (and torch.optim.AdamW); elements beside it step
+    as they would without it. In 32 bits that holds for the steps after it too."""
+    n = 2500
+    lr, wd = 1e-2, 0.0
+    grad = torch.ones(n, device=DEV)
+    runs = []
+    for value in (1.0, size):
+        p = torch.ones(n, device=DEV, dtype=pt)
+        g = grad.clone()
+        g[[5, 300, 2499]] = value
+        g[301] = -value
+        m, v, e = _state([n], bits)
+        adamw_step([p], [g], m, v, step=1, lr=lr, weight_decay=wd, exponents=e, seed=1)
+        if bits == 32:
+            assert torch.isinf(v[0]).sum() == (0 if value == 1.0 else 4)
+            runs.append(p.clone())
+            adamw_step([p], [grad], m, v, step=2, lr=lr, weight_decay=wd, exponents=e, seed=1)
+        runs.append(p.clone())
+    half = len(runs) // 2
+    big = torch.zeros(n, dtype=torch.bool, device=DEV)
+    big[[5, 300, 301, 2499]] = True
+    for ones, got in zip(runs[:half], runs[half:]):
+        assert torch.equal(got[big], torch.ones_like(got[big]))
+        assert torch.equal(got[~big], ones[~big])
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("size", [1e-15, 1e-17, 2e-18, 1e-19, 1e-20, 3e-21])
+def test_tiny_second_moments_32_bits(size, off):
+    """v down to fp32's smallest numbers, with an eps below their roots: the update is
+    the formula's of the moments as stored (their roots and quotient are within a few
+    units of 6e-8)."""
+    n = 3000
+    room = [torch.zeros(n + 1, device=DEV) for _ in range(4)]
+    p, g, m, v = (t[off: off + n] for t in room)
+    g.copy_(size * (1 + torch.rand(n, generator=gen(2))))
+    adamw_step([p], [g], [m], [v], step=1, lr=1.0, betas=(0.9, 0.999), eps=1e-30, weight_decay=0.0)
+    m64, v64 = m.double(), v.double()
+    want = -10.0 * m64 / (v64.sqrt() / 0.001 ** 0.5 + 1e-30)
+    assert (v64 > 0).all()
+    assert ((p.double() / want - 1).abs() <= 1e-6).all()
+
+
+@pytest.mark.parametrize("size", [1e-15, 1e-17, 2e-18, 1e-19, 1e-20])
+def test_tiny_second_moments_8_bits(size):
+    """The codes of small roots are those of sqrt(v), v as fp32 has it."""
+    n = 3000
+    p = torch.zeros(n, device=DEV)
+    g = (size * (1 + torch.rand(n, generator=gen(2)))).to(DEV)
+    m, v, e = _state([n], 8)
+    adamw_step([p], [g], m, v, step=1, lr=1.0, betas=(0.9, 0.999), eps=1e-30, weight_decay=0.0,
+               exponents=e, seed=7)
+    g32 = g.cpu()
+    v32 = (g32 * g32) * torch.tensor(1 - 0.999)
+    got = _values(v[0], e[1][0], 4)
+    noise = _noise(n, 7, 1, 0)
+    _close_codes(got, _rounded(v32.double().sqrt(), noise & 0xFFFF, 4, e[1][0], False), 2.0 ** -4)
+    want = -10.0 * (0.1 * g32.double()) / (v32.double().sqrt() / 0.001 ** 0.5 + 1e-30)
+    assert ((p.cpu().double() / want - 1).abs() <= 1e-6).all()
