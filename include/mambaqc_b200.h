@@ -660,12 +660,13 @@ MQC_API int mqc_adamw_moments(int64_t count, const int64_t* numel, const void* c
 MQC_API size_t mqc_grad_norm_workspace_size(int64_t count);
 
 /* Euclidean norm of all gradients together: out[0] = norm (fp32),
- * out[1] = min(1, max_norm / (norm + 1e-6)), 1 where max_norm < 0. dtype[k] is
+ * out[1] = min(1, max_norm / (norm + 1e-6)), in 64 bits and rounded once, 1 where
+ * max_norm < 0. dtype[k] is
  * the mqc_dtype of grad[k]. Fixed summation order. `workspace`: caller-owned
  * device memory, 8-byte aligned. Replaces clip_grad_norm_ (train.py:182-206)
  * without its pass that scales the gradients. */
 MQC_API int mqc_grad_norm(int64_t count, const int64_t* numel, const void* const* grad,
-                          const int32_t* dtype, float max_norm, float* out, void* workspace,
+                          const int32_t* dtype, double max_norm, float* out, void* workspace,
                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

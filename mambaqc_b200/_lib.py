@@ -217,7 +217,7 @@ _SIGNATURES.update({
     "mqc_norm_gate_bwd": [ctypes.POINTER(NormGateArgs), _c_void_p, ctypes.c_size_t, _c_void_p],
     "mqc_adamw_step": [ctypes.POINTER(AdamwArgs), _c_void_p],
     "mqc_adamw_moments": [_i64] + [_c_void_p] * 8,
-    "mqc_grad_norm": [_i64, _c_void_p, _c_void_p, _c_void_p, _f32, _c_void_p, _c_void_p,
+    "mqc_grad_norm": [_i64, _c_void_p, _c_void_p, _c_void_p, ctypes.c_double, _c_void_p, _c_void_p,
                       ctypes.c_size_t, _c_void_p],
 })
 MQC_PEER_HANDLE_BYTES = 64

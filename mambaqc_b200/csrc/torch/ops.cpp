@@ -562,7 +562,7 @@ Tensor grad_norm(const List& grads, double max_norm) {
   types.reserve(grads.size());
   for (const Tensor& g : grads) types.push_back(dtype_of(g));
   float* out = ptr<float>(all) + bytes / 4;
-  check(api.grad_norm(int64_t(grads.size()), count.data(), p.data(), types.data(), float(max_norm),
+  check(api.grad_norm(int64_t(grads.size()), count.data(), p.data(), types.data(), max_norm,
                       out, ptr(all), bytes, stream_of(all)),
         "mqc_grad_norm");
   return all.narrow(0, int64_t(bytes / 4), 2);

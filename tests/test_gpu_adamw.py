@@ -572,3 +572,17 @@ def test_tiny_second_moments_8_bits(size):
     _close_codes(got, _rounded(v32.double().sqrt(), noise & 0xFFFF, 4, e[1][0], False), 2.0 ** -4)
     want = -10.0 * (0.1 * g32.double()) / (v32.double().sqrt() / 0.001 ** 0.5 + 1e-30)
     assert ((p.cpu().double() / want - 1).abs() <= 1e-6).all()
+
+
+def test_clipping_factor_is_rounded_once():
+    """Gradients of whole numbers, whose squares add up exactly: the norm is the root
+    of a whole number, and the factor max_norm / (norm + 1e-6) has one rounding from 64
+    bits, max_norm being what the caller gave."""
+    g = gen(20)
+    for k in range(200):
+        grads = [torch.randint(-9, 10, (50 + k,), generator=g).float() for _ in range(3)]
+        norm = sum(t.double().square().sum() for t in grads).sqrt()
+        max_norm = (0.1, 1.0, 1 / 3, 0.7)[k % 4]
+        got = grad_norm([t.to(DEV) for t in grads], max_norm).cpu()
+        assert got[0] == norm.float(), k
+        assert got[1] == (max_norm / (norm + 1e-6)).float(), k
