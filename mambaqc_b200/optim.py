@@ -47,6 +47,11 @@ class AdamW(torch.optim.Optimizer):
         self.seed = seed
         self.grad_norm: torch.Tensor | None = None
 
+    def __getstate__(self) -> dict:
+        """What a copy or a pickle keeps (the base class would leave these three out)."""
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed,
+                "grad_norm": self.grad_norm}
+
     def _state_of(self, p: torch.Tensor) -> dict:
         s = self.state[p]
         if s:

@@ -170,3 +170,21 @@ def test_optimizer_refuses_without_a_gpu():
     kinds = [type(b).__name__ for b in lm.layers]
     assert kinds == ["GatedRecurrentBlock", "QuaternionMamba2Block", "GatedRecurrentBlock"]
     assert len(lm.pre_norm) == 4 and len(lm.post_norm) == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_survives_copy_and_pickle(bits):
+    import copy
+    import pickle
+
+    from mambaqc_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(300))
+    opt = AdamW([p], lr=1e-2, state_bits=bits, seed=9)
+    opt.state[p] = {"step": 3, "exp_avg": torch.ones(300), "exp_avg_sq": torch.ones(300)}
+    opt.grad_norm = torch.tensor(2.0)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.state_bits == bits and other.seed == 9 and other.grad_norm == 2.0
+        q = other.param_groups[0]["params"][0]
+        assert q is not p and other.state[q]["step"] == 3
+        assert other.param_groups[0]["lr"] == 1e-2
+        assert other.state_dict()["state_bits"] == bits
