@@ -133,8 +133,13 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Loads a state as it was saved. (The base class would cast the moments to the
-        parameters' type.)"""
-        bits = state_dict.get("state_bits", self.state_bits)
+        parameters' type.) A state of ``torch.optim.AdamW`` is one with 32-bit moments:
+        its steps become numbers, its moments flat and fp32."""
+        bits = state_dict.get("state_bits", 32)
+        for option in ("amsgrad", "maximize"):
+            if any(g.get(option) for g in state_dict["param_groups"]):
+                raise ValueError(f"AdamW: the state is one with {option}, which this optimizer "
+                                 "does not have")
         if bits != self.state_bits:
             raise ValueError(f"AdamW: the state has {bits}-bit moments, "
                              f"the optimizer {self.state_bits}-bit ones")
@@ -144,6 +149,10 @@ class AdamW(torch.optim.Optimizer):
         params = [p for g in self.param_groups for p in g["params"]]
         for k, p in zip(places, params):
             for name, value in state_dict["state"].get(k, {}).items():
-                if torch.is_tensor(value):
-                    value = value.detach().to(p.device, copy=True)
+                if name == "step":
+                    value = int(value)
+                elif torch.is_tensor(value):
+                    value = value.detach().reshape(-1)      # in the order of p's elements
+                    dtype = torch.float32 if value.is_floating_point() else value.dtype
+                    value = value.to(p.device, dtype, copy=True)
                 self.state[p][name] = value

@@ -586,3 +586,36 @@ def test_clipping_factor_is_rounded_once():
         got = grad_norm([t.to(DEV) for t in grads], max_norm).cpu()
         assert got[0] == norm.float(), k
         assert got[1] == (max_norm / (norm + 1e-6)).float(), k
+
+
+def test_continues_a_state_of_torch_adamw(monkeypatch):
+    """The steps after the switch are those of torch's optimizer, one call each."""
+    from mambaqc_b200 import optim
+
+    def params():
+        g = gen(31)
+        return [torch.nn.Parameter(torch.randn(s, generator=g).to(DEV)) for s in ((20, 30), (7,))] \
+            + [torch.nn.Parameter(torch.randn(8, 5, generator=g).to(DEV).t())]
+
+    def steps(opt, which, ps):
+        for k in which:
+            g = gen(200 + k)
+            for p in ps:
+                p.grad = torch.randn(p.shape, generator=g).to(DEV)
+            opt.step()
+
+    a = params()
+    oa = torch.optim.AdamW(a, lr=1e-2, weight_decay=0.1)
+    steps(oa, range(4), a)
+    b = params()
+    for p, q in zip(a, b):
+        q.data.copy_(p.data)
+    ob = AdamW(b)
+    ob.load_state_dict(oa.state_dict())
+    calls = []
+    monkeypatch.setattr(optim, "adamw_step", lambda *x, **k: calls.append(1) or adamw_step(*x, **k))
+    steps(oa, range(4, 8), a)
+    steps(ob, range(4, 8), b)
+    assert len(calls) == 4
+    for p, q in zip(a, b):
+        assert rel_l2(q, p) < 8e-6

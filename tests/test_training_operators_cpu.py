@@ -188,3 +188,40 @@ def test_optimizer_survives_copy_and_pickle(bits):
         assert q is not p and other.state[q]["step"] == 3
         assert other.param_groups[0]["lr"] == 1e-2
         assert other.state_dict()["state_bits"] == bits
+
+
+def test_state_of_torch_adamw_loads():
+    """Steps as numbers (parameters that share one are stepped in one call), moments
+    flat in the parameters' order and fp32; what has no counterpart is refused."""
+    from mambaqc_b200.optim import AdamW
+
+    def params():
+        g = torch.Generator().manual_seed(3)
+        return [torch.nn.Parameter(torch.randn(5, 7, generator=g)),
+                torch.nn.Parameter(torch.randn(6, 4, generator=g).t()),
+                torch.nn.Parameter(torch.randn(9, generator=g).bfloat16())]
+
+    theirs = params()
+    opt = torch.optim.AdamW(theirs, lr=1e-2, betas=(0.8, 0.9))
+    for _ in range(3):
+        for p in theirs:
+            p.grad = torch.randn(p.shape).to(p.dtype)
+        opt.step()
+    ours = params()
+    got = AdamW(ours)
+    got.load_state_dict(opt.state_dict())
+    assert got.param_groups[0]["lr"] == 1e-2 and tuple(got.param_groups[0]["betas"]) == (0.8, 0.9)
+    for p, q in zip(theirs, ours):
+        s, want = got.state[q], opt.state[p]
+        assert type(s["step"]) is int and s["step"] == 3
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert s[name].dtype == torch.float32 and s[name].is_contiguous()
+            assert torch.equal(s[name], want[name].float().reshape(-1))
+    again = AdamW(params())
+    again.load_state_dict(got.state_dict())
+    assert all(type(again.state[q]["step"]) is int for q in again.param_groups[0]["params"])
+    with pytest.raises(ValueError, match="32-bit"):
+        AdamW(params(), state_bits=8).load_state_dict(opt.state_dict())
+    odd = torch.optim.AdamW(params(), amsgrad=True)
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW(params()).load_state_dict(odd.state_dict())
