@@ -97,8 +97,7 @@ class AdamW(torch.optim.Optimizer):
         calls: dict[tuple, list] = {}
         for group, place, p, g in work:
             s = self._state_of(p)
-            s["step"] += 1
-            key = (id(group), s["step"], p.device)
+            key = (id(group), s["step"] + 1, p.device)
             calls.setdefault(key, [group]).append((place, p, g, s))
         for (_, step, device), (group, *members) in calls.items():
             dense = [p if p.is_contiguous() else p.contiguous() for _, p, _, _ in members]
@@ -112,7 +111,8 @@ class AdamW(torch.optim.Optimizer):
                        betas=group["betas"], eps=group["eps"],
                        weight_decay=group["weight_decay"], exponents=exponents, seed=self.seed, carry=True,
                        clip=clips.get(device), ordinals=[k for k, _, _, _ in members])
-            for d, (_, p, _, _) in zip(dense, members):
+            for d, (_, p, _, s) in zip(dense, members):
+                s["step"] = step        # counted when done: not by a call that is refused
                 if d is not p:
                     p.copy_(d)
         return loss

@@ -225,3 +225,14 @@ def test_state_of_torch_adamw_loads():
     odd = torch.optim.AdamW(params(), amsgrad=True)
     with pytest.raises(ValueError, match="amsgrad"):
         AdamW(params()).load_state_dict(odd.state_dict())
+
+
+def test_refused_step_is_not_counted():
+    from mambaqc_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(4))
+    p.grad = torch.ones(4)
+    opt = AdamW([p])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            opt.step()
+    assert opt.state[p]["step"] == 0
