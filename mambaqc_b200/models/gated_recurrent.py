@@ -61,12 +61,17 @@ class GatedRecurrentBlock(nn.Module):
         packed sequence (the recurrence drops its state there; the conv still sees up
         to d_conv - 1 tokens before it)."""
         x_in, z = self._project(x)
+        y, h_T = self._recur(x_in, reset)
+        return y, z, h_T
+
+    def _recur(self, x_in: torch.Tensor, reset: torch.Tensor | None = None):
+        """(y, h_T) from the projected input."""
         conv = self.conv1d.conv
         x_act = causal_conv1d_silu(x_in, conv.weight, conv.bias)
         r, i = self.gate_proj(x_act).to(x_act.dtype).chunk(2, dim=-1)
         h, h_T = gated_linear_scan(x_act, r, i, self.Lambda, None, reset,
                                    sharpness=self.sharpness, return_final_state=True)
-        return self.out_proj(h), z, h_T
+        return self.out_proj(h), h_T
 
     def forward(self, x: torch.Tensor, reset: torch.Tensor | None = None):
         return self.mix(x, reset)[:2]
@@ -75,9 +80,9 @@ class GatedRecurrentBlock(nn.Module):
     def mix_prefill(self, x: torch.Tensor):
         """``mix`` over a prompt with the cache a continuation needs: the last d_conv - 1
         conv inputs and the fp32 state."""
-        y, z, h_T = self.mix(x)
+        x_in, z = self._project(x)
+        y, h_T = self._recur(x_in)
         k1 = self.d_conv - 1
-        x_in = self._project(x)[0]
         hist = x_in.new_zeros(x.shape[0], k1, self.d_inner)
         take = min(k1, x.shape[1])
         if take > 0:

@@ -147,3 +147,19 @@ def test_refusals():
         HybridMamba2(V, d_model=DM, n_layers=2, pattern="gx")
     with pytest.raises(AssertionError, match="norm"):
         HybridMamba2(V, d_model=DM, n_layers=2, norm="batch")
+
+
+def test_prefill_projects_the_prompt_once():
+    torch.manual_seed(0)
+    block = GatedRecurrentBlock(DM).to(DEV)
+    x = torch.randn(2, 9, DM, generator=gen(3)).to(DEV)
+    calls = []
+    block.in_proj.register_forward_hook(lambda *_: calls.append(1))
+    with torch.no_grad():
+        y, z, cache = block.mix_prefill(x)
+        assert len(calls) == 1
+        want = block.mix(x)
+        x_in = block.in_proj(x)[..., : block.d_inner]
+    for a, b in zip((y, z, cache["h"]), want):
+        assert torch.equal(a, b)
+    assert torch.equal(cache["conv"], x_in[:, -(block.d_conv - 1):])
