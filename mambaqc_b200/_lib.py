@@ -293,8 +293,8 @@ def torch_ops():
                     from . import _torch_ops as ops
                 except ImportError as e:
                     raise RuntimeError(
-                        "mambaqc_b200: the torch extension is not built; run "
-                        "`python -m mambaqc_b200.csrc.build`") from e
+                        "mambaqc_b200: the torch extension is not built, or not for this "
+                        "torch and Python; run `python -m mambaqc_b200.csrc.build`") from e
                 ops.init(str(LIB_PATH))
                 _torch_ops = ops
     return _torch_ops

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -97,23 +98,39 @@ def build(force: bool = False, jobs: int | None = None, quiet: bool = False) -> 
     return LIB
 
 
-def build_torch_ops(force: bool = False, quiet: bool = False) -> Path:
-    """The torch extension; compiled again when its source or the header is newer."""
+def build_torch_ops(force: bool = False, quiet: bool = False) -> Path | None:
+    """The torch extension; compiled again when its source or the header is newer, or
+    when it was built for another torch or Python. None, with a message, where torch, its
+    headers or g++ are missing: the C library does without them."""
+    missing = None
+    if importlib.util.find_spec("torch") is None:
+        missing = "torch"
+    elif shutil.which("g++") is None:
+        missing = "g++"
+    else:
+        import torch
+
+        root = Path(torch.__file__).resolve().parent
+        if not (root / "include" / "torch" / "extension.h").exists():
+            missing = "torch's headers"
+    if missing:
+        print(f"{OPS_LIB.name} is not built: no {missing} (the C library is; the operators of "
+              "the training stack need both)", file=sys.stderr)
+        return None
+    built_for = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
     newest = max(p.stat().st_mtime for p in (OPS_SOURCE, INCLUDE / "mambaqc_b200.h"))
-    if not force and OPS_LIB.exists() and OPS_LIB.stat().st_mtime >= newest:
+    if not force and OPS_LIB.exists() and OPS_LIB.stat().st_mtime >= newest \
+            and f"mqc built for {built_for};".encode() in OPS_LIB.read_bytes():
         return OPS_LIB
     import sysconfig
 
-    import torch
-
-    root = Path(torch.__file__).resolve().parent
     cuda_home = Path(_nvcc()).resolve().parents[1]
     include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
                cuda_home / "include", Path(sysconfig.get_paths()["include"]), INCLUDE]
     tmp = OPS_LIB.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_torch_ops", *[f"-I{p}" for p in include], str(OPS_SOURCE),
+           "-DTORCH_EXTENSION_NAME=_torch_ops", f'-DMQC_BUILT_FOR="mqc built for {built_for};"', *[f"-I{p}" for p in include], str(OPS_SOURCE),
            "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_cuda", "-ltorch", "-ltorch_python", "-ldl"]
     proc = subprocess.run(cmd, capture_output=True, text=True)

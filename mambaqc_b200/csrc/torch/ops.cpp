@@ -640,6 +640,7 @@ std::tuple<List, List> adamw_moments(const List& m, const List& v, const List& e
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, mod) {
+  mod.attr("built_for") = MQC_BUILT_FOR;  // what csrc/build.py looks for in this file
   mod.def("init", &init);
   mod.def("gated_scan", &gated_scan);
   mod.def("gated_step", &gated_step);

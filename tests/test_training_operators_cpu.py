@@ -236,3 +236,31 @@ def test_refused_step_is_not_counted():
         with pytest.raises(RuntimeError, match="CUDA"):
             opt.step()
     assert opt.state[p]["step"] == 0
+
+
+def test_extension_is_built_again_for_another_torch(monkeypatch, tmp_path, capsys):
+    """An extension newer than its source, but for another torch, is compiled again;
+    without torch's headers or g++ the C library is built alone."""
+    import shutil
+    import subprocess
+
+    from mambaqc_b200.csrc import build
+    _lib.torch_ops()                                        # this one loads
+    lib = tmp_path / "_torch_ops.so"
+    shutil.copy(build.OPS_LIB, lib)
+    monkeypatch.setattr(build, "OPS_LIB", lib)
+    ran = []
+
+    def run(cmd, **_):
+        ran.append(cmd)
+        lib.with_suffix(".so.tmp").write_bytes(b"new")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    assert build.build_torch_ops(quiet=True) == lib and not ran
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    assert build.build_torch_ops(quiet=True) == lib and len(ran) == 1
+    assert lib.read_bytes() == b"new"
+    monkeypatch.setattr(build.shutil, "which", lambda name: None)
+    assert build.build_torch_ops(force=True, quiet=True) is None and len(ran) == 1
+    assert "no g++" in capsys.readouterr().err
