@@ -10,7 +10,8 @@ from tests.gpu_util import DEV, RTOL_F32, gen, rel_l2
 
 pytestmark = pytest.mark.gpu
 
-from mambaqc_b200.kernels import gate_residual  # noqa: E402
+from mambaqc_b200.kernels import (gate_residual, gated_linear_scan, gated_linear_step,  # noqa: E402
+                                  norm_gate_residual, residual_norm)
 from mambaqc_b200.models import (GatedRecurrentBlock, HybridMamba2,  # noqa: E402
                                  QuaternionMamba2Block)
 from mambaqc_b200.optim import AdamW  # noqa: E402
@@ -163,3 +164,38 @@ def test_prefill_projects_the_prompt_once():
     for a, b in zip((y, z, cache["h"]), want):
         assert torch.equal(a, b)
     assert torch.equal(cache["conv"], x_in[:, -(block.d_conv - 1):])
+
+
+def test_operators_in_a_captured_graph():
+    """Recurrence, its one-token form and the norms, forward, replay on new inputs from a
+    CUDA graph with the bits of the calls."""
+    b, t, d = 2, 300, 64
+    g = gen(17)
+    lam = torch.randn(d, generator=g).to(DEV) - 4
+    w = torch.rand(d, generator=g).to(DEV) + 0.5
+    x, r, i, z = (torch.randn(b, t, d, generator=g).to(DEV) for _ in range(4))
+    h = torch.zeros(b, d, device=DEV)
+
+    def run(state):
+        y, h_T = gated_linear_scan(x, r, i, lam, return_final_state=True)
+        out, n = norm_gate_residual(x, y, z, w, w, next_weight=w)
+        state.copy_(h_T)
+        step = gated_linear_step(x[:, 0], r[:, 0], i[:, 0], lam, state)
+        return y, out, n, residual_norm(out, w), step
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(h)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(h)
+        for k in range(2):
+            for v in (x, r, i, z):
+                v.copy_(torch.randn(b, t, d, generator=g))
+            graph.replay()
+            want = run(torch.zeros(b, d, device=DEV))
+            for a, e in zip(got, want):
+                assert torch.equal(a, e), k
