@@ -12,8 +12,8 @@
 // Layout. A CTA owns 64 channels of one sequence and walks over time in tiles of
 // 32 or 64 steps; each warp takes a run of consecutive steps of the tile, each lane
 // two channels, so the arithmetic is packed two-wide; the tile's rows come through
-// shared memory (cp.async). A run is reduced to (A, E), h_out = A h_in + E (held as
-// A - 1), in registers; runs are joined through shared memory, tiles through the
+// shared memory (cp.async). A run is reduced to (A, E), h_out = A h_in + E (A held as
+// A - 1 from 1/2 up), in registers; runs are joined through shared memory, tiles through the
 // shared memory of a thread-block cluster whose CTAs take consecutive tiles of the same
 // sequence. So each input is read once and each output written once, and no CTA waits
 // for another one outside its cluster.
@@ -22,11 +22,12 @@
 // the forward pass left at the tile's start (y in bf16 would cost dLambda three
 // digits), and the reverse recurrence uses the same products A.
 //
-// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 34 us, backward 69 us (and 3 for
+// Measured, bf16, 4 x 2048 x 1536 on one B200: forward 35 us, backward 68 us (and 3 for
 // dLambda), where the bytes alone take 15 and 27 us at 6.5 TB/s; 1 x 32768 x 1024
-// forward 124 us (41): a round of the cluster takes 2.15 us with one CTA an SM, 3.1
-// with two and 4 with three, and clusters of 16 come to three on some SMs. Found at
-// 35.3 us, before the short form of slow decays: neither memory bounds the forward (with
+// forward 129 us (41), backward 231: a round of the cluster takes 2.15 us with one CTA an
+// SM, 3.1 with two and 4 with three, and clusters of 16 come to three on some SMs. With
+// products of decays held as A - 1 throughout it was 34, 69, 125 and 223. Found at
+// 35.3 us, before that and the short form of slow decays: neither memory bounds the forward (with
 // all tiles read from the cache and nothing stored it took 34 us) nor the special
 // functions (35 us without any) nor one pipe (the fullest, FMA, 46 % busy), but the
 // phases of a tile between barriers: 47 instructions an element at 0.57 a cycle and
@@ -68,10 +69,13 @@ constexpr int kChan = 64;  // channels of a CTA
 constexpr int kBwdTile = MQC_GATED_SCAN_TILE;  // time steps of a tile backward, and of a checkpoint
 constexpr int kRun = 8;  // steps of a warp's run forward
 // Forward, sequences of up to kShort steps go in tiles of 32 (four warps), longer ones
-// in tiles of 64 (eight). bf16, us with 32 and 64: 512 x 64 x 1024 66.5 and 86.2, 256 x
-// 128 x 1024 63 and 73, 64 x 512 x 1024 72 and 68, 4 x 2048 x 1536 33.3 and 34.2, 1 x
-// 32768 x 1024 147 and 127: small CTAs hide one another's loads where a sequence is done
-// in a round or two, large ones take half the rounds where it is long.
+// in tiles of 64 (eight). us with 32 and 64, bf16 (fp32): 512 x 64 x 1024 65 and 85 (89
+// and 121), 256 x 128 x 1024 62 and 73 (85 and 102), 1 x 32768 x 1024 153 and 129 (224 and
+// 190), 1 x 8192 x 1024 41 and 36 (59 and 50): small CTAs hide one another's loads where a
+// sequence is done in a round or two, large ones take half the rounds where it is long.
+// Between, neither is better throughout: 200 x 160 x 1024 60 and 83 (85 and 109), 24 x 320
+// x 768 19 and 16 (both 19), 40 x 300 x 1024 39 and 32 (51 and 44), 64 x 512 x 1024 75 and
+// 67 (87 and 96), 4 x 2048 x 1536 both 34 (40 and 51), 1 x 2048 x 1536 both 15 (23 and 16).
 constexpr int kShort = 128;
 // CTAs of a cluster: as many as the exchange's shared memory leaves room for two CTAs
 // an SM beside (16 is the device's limit, above the portable 8)
@@ -168,8 +172,8 @@ __device__ __forceinline__ void decay2(float2 v, float2& a, float2& m, float2& q
 // by to -L. As s(r) <= 1, a warp whose rates are all within kNear needs no reduction of
 // the exponent (small_rates): decays of 0.7 a step and slower,
 // which is where such layers start and mostly stay. Forward, slow against fast decays:
-// 33.7 and 35.8 us at 4 x 2048 x 1536, 124 and 134 at 1 x 32768 x 1024; backward 69 and
-// 70.8, 223 and 237.
+// 34.9 and 36.9 us at 4 x 2048 x 1536, 129 and 139 at 1 x 32768 x 1024; backward 68.2 and
+// 70.4, 231 and 241.
 __device__ __forceinline__ float2 neg_rate2(float2 lam, float sharpness, bool ok0, bool ok1) {
   return make_float2(ok0 ? -sharpness * softplus_acc(lam.x) : 0.f, ok1 ? -sharpness * softplus_acc(lam.y) : 0.f);
 }
@@ -911,9 +915,15 @@ void ask_fit(K kernel, int threads, size_t smem, int most, Fit& fit) {
 // What a round of a tile takes in a wave of clusters, in units of what each CTA that
 // shares the SM adds to it: `latency`, and the exchange between up to `few` CTAs or more.
 // Fitted to bf16 at nine shapes and cluster sizes 1 to 16; us at the sizes 1, 2, 4, 8:
-//   forward (units of 0.8 us)     4 x 2048 x 1536  62, 48, 35, -   64 x 512 x 1024  72, 81, 101, -
-//   backward (units of 0.88 us)   4 x 2048 x 1536  89, 82, 71, 75  64 x 512 x 1024  127, 154, 185, 255
-//                                 6 x 2048 x 1536  91, 83, 108, 111
+//   forward (units of 0.8 us)     4 x 2048 x 1536  66, 48, 35, 40  64 x 512 x 1024  68, 79, 100, 145
+//   backward (units of 0.88 us)   4 x 2048 x 1536  84, 80, 68, 73  64 x 512 x 1024  120, 149, 180, 252
+//                                 6 x 2048 x 1536  87, 80, 105, 108
+// fp32 (sizes up to 8) goes by the same numbers: 4 x 2048 x 1536 forward 78, 52, 51, 52,
+// backward 104, 92, 80, 84. Against every size at 16 shapes (1 to 512 sequences of 64 to
+// 32768 steps) the size taken is within 3 % of the best in 29 of 32 bf16 and 26 of 32 fp32
+// launches; farthest off: 32 x 100 x 512 forward 9.1 and 7.9 us, 3 x 2048 x 1536 forward
+// 33 and 31, fp32 46 and 39, 8 x 512 x 1536 backward 39 and 36, 1 x 32768 x 1024 backward,
+// fp32, 366 and 340.
 struct RoundCost {
   double latency, exchange_few, exchange_more;
   int few;

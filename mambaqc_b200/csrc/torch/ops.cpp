@@ -4,8 +4,10 @@
 //
 // The other operators are bound with ctypes and torch.autograd.Function. A Python
 // autograd function costs 100 us and more of host time for a forward and a backward
-// with eight inputs, which is above what the kernels take at most sizes; this one costs
-// what a built-in operator does. It holds no kernels and no state: arguments are
+// with eight inputs and nothing inside, which is above what the kernels take at most
+// sizes. Small tensors, forward and backward in a loop: the recurrence (four inputs with
+// a gradient) 79 us, the norm (eight) 115, a built-in layer norm (two) 73, a product of
+// two tensors 60. It holds no kernels and no state: arguments are
 // checked in Python (kernels/*.py) before they come here, memory is torch's, and
 // failures of the C ABI become RuntimeErrors with its message.
 #include <ATen/cuda/CUDAContext.h>
