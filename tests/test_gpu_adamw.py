@@ -619,3 +619,17 @@ def test_continues_a_state_of_torch_adamw(monkeypatch):
     assert len(calls) == 4
     for p, q in zip(a, b):
         assert rel_l2(q, p) < 8e-6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_smallest_eps(bits):
+    """An eps that has no fp32 reciprocal: parameters whose gradients are all zero stay
+    where they are, the others step by the formula."""
+    n = 700
+    grad = torch.zeros(n, device=DEV)
+    grad[1::2] = 3.0
+    p = torch.ones(n, device=DEV)
+    m, v, e = _state([n], bits)
+    adamw_step([p], [grad], m, v, step=1, lr=1e-2, eps=1e-40, weight_decay=0.0, exponents=e)
+    assert torch.equal(p[0::2], torch.ones_like(p[0::2]))
+    assert ((p[1::2] - 0.99).abs() < 1e-6).all()
