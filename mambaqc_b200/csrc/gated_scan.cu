@@ -39,7 +39,8 @@
 // long prefill 129 against 133).
 //
 // Backward, tiles of 32 steps: the barriers of two CTAs an SM overlap, where one CTA of
-// 16 warps and tiles of 64 took 79 us (512 x 64 x 1024: 160 against 253). Slower: three
+// 16 warps and tiles of 64 took 79 us (512 x 64 x 1024: 160 against 253; only 3 x 2048 x
+// 1536 was faster with it, 50 us against 58, now 56). Slower: three
 // CTAs an SM at 85 registers (78 us); and with tiles of 64, eight warps of eight steps
 // (82 us), one joining warp of channel pairs (94 us), the states' half of the second
 // pass under the exchange for one more barrier (81 us; 64 x 512 x 1024 170 against 154).
